@@ -382,6 +382,62 @@ int miq_linear_dynamic_w8a8(const void* x, int x_dtype, const int8_t* W, int64_t
                             const float* w_scale, const float* bias, const float* w_rowsum, void* out, int out_dtype,
                             void* workspace, size_t workspace_bytes, unsigned* counter, void* stream);
 
+/* ---- block-scaled 8-bit floating point -------------------------------------------------------------------------
+ *
+ * Codes are OCP e4m3 (largest value 448), one byte each; the value of a code is code * scale.  A block is 128 consecutive
+ * columns, the last one of a row may be shorter.  Activations [M,K] have a scale for each row and block, held block-major:
+ * scale[b * M + m], b < ceil(K / 128).  Weights [N,K] have one for each block of 128 x 128: scale[(n / 128) * ceil(K / 128)
+ * + b].  All scales are fp32.  The reference has no 8-bit floating point and no scale finer than a tensor or a channel
+ * (quant/Weight_Only/Qop.py:104-137 sketches groups, and raises); these operators stand next to the int8 path, with its
+ * conventions.
+ *
+ * With a = max(largest finite |x| of the block, 448 * 2^-126):
+ *     scale = a / 448        q = e4m3(x * (448 / a))        (fp32; the quotients are IEEE divisions, one of each per block;
+ *                                                            the conversion rounds half to even)
+ * A value that is not finite becomes the NaN code and does not enter its block's maximum.
+ *
+ * Outputs must not overlap inputs.  A call whose launch would pass 2^32 threads returns MIQ_ERANGE (from 2^22 rows of more than
+ * 8192 columns, 2^24 of fewer, or 2^24 blocks of 128 x 128). */
+
+/* Activations to codes: x [M,K] of x_dtype MIQ_F32 | MIQ_F16 | MIQ_BF16 -> q [M,K], scale [ceil(K/128), M]. */
+int miq_quantize_blocks_fp8(const void* x, int x_dtype, int64_t M, int64_t K, uint8_t* q, float* scale, void* stream);
+
+/* Weights to codes: w [N,K] of w_dtype -> q [N,K], scale [ceil(N/128), ceil(K/128)]. */
+int miq_quantize_weight_fp8(const void* w, int w_dtype, int64_t N, int64_t K, uint8_t* q, float* scale, void* stream);
+
+/* Root-mean-square norm with the residual's addition, to codes:
+ *     h = x + residual (rounded to dtype; h = x without a residual)       sum = h (written when there is a residual)
+ *     y[m,k] = (h[m,k] * (1 / sqrt(mean_k h[m,k]^2 + eps))) * weight[k]   fp32
+ *     q, scale = the codes of y
+ * x, residual, sum: [M,K] of dtype; residual and sum are both null or both given.  weight: [K] of weight_dtype, which is
+ * dtype or MIQ_F32. */
+int miq_rms_norm_fp8(const void* x, const void* residual, const void* weight, int dtype, int weight_dtype, int64_t M, int64_t K,
+                     float eps, void* sum, uint8_t* q, float* scale, void* stream);
+
+/* Linear on codes:
+ *     out[m,n] = sum_b (x_scale[b,m] * w_scale[n/128,b]) * (sum_{k in block b} x[m,k] * w[n,k]) + bias[n]
+ * x [M,K] and w [N,K] are codes with their scales in the layouts above; bias fp32 [N] or NULL; out [M,N] of out_dtype
+ * MIQ_F32 | MIQ_F16 | MIQ_BF16, 16-byte aligned.  Products and sums are fp32, rounded once to out_dtype.  Any K and any
+ * alignment of x and w; a multiple of 16 on 16-byte aligned operands is staged without passing through registers.
+ * The product of two scales has to be a finite fp32 number.
+ * M, N below 2^31, K below 2^22, at most 2^22 tiles of 64 x 64 outputs (MIQ_ERANGE otherwise).
+ * workspace: at least miq_gemm_fp8_workspace(...) bytes, 256-byte aligned; may be NULL when that is 0. */
+size_t miq_gemm_fp8_workspace(int64_t M, int64_t N, int64_t K);
+int miq_gemm_fp8(const uint8_t* x, const float* x_scale, const uint8_t* w, const float* w_scale, int64_t M, int64_t N, int64_t K,
+                 const float* bias, void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gated Linear on codes, the first half of a gated feed-forward block:
+ *     g = x . w_gate^T      u = x . w_up^T      (the sums of miq_gemm_fp8, kept in fp32)
+ *     q, scale = the codes of act(g) * u        [M,N], [ceil(N/128), M]
+ * act: MIQ_ACT_SILU  g / (1 + exp(-g)),  MIQ_ACT_GELU  g / 2 * (1 + erf(g / sqrt(2))).
+ * w_gate and w_up are [N,K] codes with scales of their own.  Sizes and workspace as for miq_gemm_fp8. */
+#define MIQ_ACT_SILU 0
+#define MIQ_ACT_GELU 1
+size_t miq_gated_fp8_workspace(int64_t M, int64_t N, int64_t K);
+int miq_gated_fp8(const uint8_t* x, const float* x_scale, const uint8_t* w_gate, const float* gate_scale, const uint8_t* w_up,
+                  const float* up_scale, int64_t M, int64_t N, int64_t K, int act, uint8_t* q, float* scale, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

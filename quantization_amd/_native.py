@@ -17,6 +17,7 @@ MIQ_F32, MIQ_F16, MIQ_BF16, MIQ_I32, MIQ_I8 = 0, 1, 2, 3, 4
 MIQ_POOL_MAX, MIQ_POOL_AVG = 0, 1
 MIQ_W_NK, MIQ_W_KN = 0, 1
 MIQ_OUT_MN, MIQ_OUT_NM = 0, 1
+MIQ_ACT_SILU, MIQ_ACT_GELU = 0, 1
 
 _FLOAT_CODES = {torch.float32: MIQ_F32, torch.float16: MIQ_F16, torch.bfloat16: MIQ_BF16}
 _OUT_CODES = {torch.float32: MIQ_F32, torch.bfloat16: MIQ_BF16, torch.int32: MIQ_I32}
@@ -70,6 +71,13 @@ SYMBOLS = {
     "miq_dynamic_quant_params_i8": (_int, [_p, _int, _i64, _p, _p, _p, _i64, _p, _p, _p, _p, _size, _p, _p]),
     "miq_quantize_tensor_i8": (_int, [_p, _int] + [_i64] * 7 + [_p, _p, _p]),
     "miq_dynamic_quantize_i8": (_int, [_p, _int] + [_i64] * 7 + [_p, _p, _p, _i64, _p, _p, _p, _p, _p, _size, _p, _p]),
+    "miq_quantize_blocks_fp8": (_int, [_p, _int, _i64, _i64, _p, _p, _p]),
+    "miq_quantize_weight_fp8": (_int, [_p, _int, _i64, _i64, _p, _p, _p]),
+    "miq_rms_norm_fp8": (_int, [_p, _p, _p, _int, _int, _i64, _i64, ctypes.c_float, _p, _p, _p, _p]),
+    "miq_gemm_fp8_workspace": (_size, [_i64] * 3),
+    "miq_gemm_fp8": (_int, [_p] * 4 + [_i64] * 3 + [_p, _p, _int, _p, _size, _p]),
+    "miq_gated_fp8_workspace": (_size, [_i64] * 3),
+    "miq_gated_fp8": (_int, [_p] * 6 + [_i64] * 3 + [_int, _p, _p, _p, _size, _p]),
     "miq_linear_dynamic_w8a8_workspace": (_size, [_i64] * 3),
     "miq_linear_dynamic_w8a8": (_int, [_p, _int, _p] + [_i64] * 3 + [_p, _p, _p, _p, _int, _p, _size, _p, _p]),
 }
@@ -779,3 +787,127 @@ def epilogue_channels_f32(y, bias, alpha, beta=0.0):
         _check(lib().miq_epilogue_channels_f32(_ptr(y), _ptr(bias), _ptr(alpha), float(beta), outer, channels,
                                                inner, _ptr(out), _stream()))
     return out
+
+
+# ---- block-scaled 8-bit floating point ------------------------------------------------------------------------------
+
+_F8 = torch.float8_e4m3fn
+_FP8_OUT_CODES = _FLOAT_CODES
+_ACT_CODES = {"silu": MIQ_ACT_SILU, "gelu": MIQ_ACT_GELU}
+
+
+def _require_same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise RuntimeError(f"{name} must be on {device} (got {t.device})")
+
+
+def _fp8_matrix(q, scale, name, scale_shape):
+    """Checks a matrix of codes and its scales; returns (rows, columns)."""
+    require_device(q, name)
+    require_device(scale, f"the scales of {name}")
+    if q.dtype != _F8 or q.dim() != 2:
+        raise RuntimeError(f"{name} must be a float8_e4m3fn matrix, got {tuple(q.shape)} {q.dtype}")
+    if scale.dtype != torch.float32 or tuple(scale.shape) != scale_shape(*q.shape):
+        raise RuntimeError(f"the scales of {name} {tuple(q.shape)} must be float32 {scale_shape(*q.shape)}, got {tuple(scale.shape)} {scale.dtype}")
+    return q.shape
+
+
+def _act_scale_shape(m, k):
+    return ((k + 127) // 128, m)
+
+
+def _weight_scale_shape(n, k):
+    return ((n + 127) // 128, (k + 127) // 128)
+
+
+def _float_matrix(x, name):
+    require_device(x, name)
+    if x.dtype not in _FLOAT_CODES or x.dim() != 2:
+        raise RuntimeError(f"{name} must be a float32, float16 or bfloat16 matrix, got {tuple(x.shape)} {x.dtype}")
+    return x.shape
+
+
+def quantize_blocks_fp8(x):
+    """x [M, K] float -> (codes float8_e4m3fn [M, K], scales fp32 [ceil(K / 128), M])."""
+    M, K = _float_matrix(x, "input")
+    q = torch.empty((M, K), dtype=_F8, device=x.device)
+    scale = torch.empty(_act_scale_shape(M, K), dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        _check(lib().miq_quantize_blocks_fp8(_ptr(x), _FLOAT_CODES[x.dtype], M, K, _ptr(q), _ptr(scale), _stream()))
+    return q, scale
+
+
+def quantize_weight_fp8(w):
+    """w [N, K] float -> (codes float8_e4m3fn [N, K], scales fp32 [ceil(N / 128), ceil(K / 128)])."""
+    N, K = _float_matrix(w, "weight")
+    q = torch.empty((N, K), dtype=_F8, device=w.device)
+    scale = torch.empty(_weight_scale_shape(N, K), dtype=torch.float32, device=w.device)
+    with _on(w.device):
+        _check(lib().miq_quantize_weight_fp8(_ptr(w), _FLOAT_CODES[w.dtype], N, K, _ptr(q), _ptr(scale), _stream()))
+    return q, scale
+
+
+def rms_norm_fp8(x, weight, eps, residual=None):
+    """x [M, K] float -> (codes, scales, x + residual or None)."""
+    M, K = _float_matrix(x, "input")
+    require_device(weight, "weight")
+    if tuple(weight.shape) != (K,) or weight.dtype not in (x.dtype, torch.float32):
+        raise RuntimeError(f"weight must be [{K}] of {x.dtype} or float32, got {tuple(weight.shape)} {weight.dtype}")
+    total = None
+    if residual is not None:
+        require_device(residual, "residual")
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise RuntimeError(f"residual must be {tuple(x.shape)} {x.dtype}, got {tuple(residual.shape)} {residual.dtype}")
+        total = torch.empty_like(x)
+    _require_same_device(x.device, weight=weight, residual=residual)
+    q = torch.empty((M, K), dtype=_F8, device=x.device)
+    scale = torch.empty(_act_scale_shape(M, K), dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        _check(lib().miq_rms_norm_fp8(_ptr(x), _ptr(residual), _ptr(weight), _FLOAT_CODES[x.dtype], _FLOAT_CODES[weight.dtype], M, K,
+                                      eps, _ptr(total), _ptr(q), _ptr(scale), _stream()))
+    return q, scale, total
+
+
+def gemm_fp8(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16):
+    """Codes x [M, K] times codes w [N, K]^T, each with its block scales, plus bias -> [M, N] of out_dtype."""
+    M, K = _fp8_matrix(x, x_scale, "input", _act_scale_shape)
+    N, Kw = _fp8_matrix(w, w_scale, "weight", _weight_scale_shape)
+    if K != Kw:
+        raise RuntimeError(f"input has {K} columns, weight {Kw}")
+    if out_dtype not in _FP8_OUT_CODES:
+        raise RuntimeError(f"unsupported output dtype {out_dtype}")
+    dev = x.device
+    _require_same_device(dev, x_scale=x_scale, weight=w, w_scale=w_scale)
+    bias = _f32_vec(bias, N, "bias", dev)
+    out = torch.empty((M, N), dtype=out_dtype, device=dev)
+    L = lib()
+    need = L.miq_gemm_fp8_workspace(M, N, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    with _on(dev):
+        _check(L.miq_gemm_fp8(_ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), M, N, K, _ptr(bias), _ptr(out),
+                              _FP8_OUT_CODES[out_dtype], _ptr(ws), need, _stream()))
+    return out
+
+
+def gated_fp8(x, x_scale, w_gate, gate_scale, w_up, up_scale, act="silu"):
+    """Codes of act(x . w_gate^T) * (x . w_up^T): (codes [M, N], scales [ceil(N / 128), M])."""
+    M, K = _fp8_matrix(x, x_scale, "input", _act_scale_shape)
+    N, Kg = _fp8_matrix(w_gate, gate_scale, "gate weight", _weight_scale_shape)
+    if K != Kg:
+        raise RuntimeError(f"input has {K} columns, gate weight {Kg}")
+    if _fp8_matrix(w_up, up_scale, "up weight", _weight_scale_shape) != w_gate.shape:
+        raise RuntimeError(f"gate weight is {tuple(w_gate.shape)}, up weight {tuple(w_up.shape)}")
+    if act not in _ACT_CODES:
+        raise RuntimeError(f"unknown activation {act!r}: silu or gelu")
+    dev = x.device
+    _require_same_device(dev, x_scale=x_scale, w_gate=w_gate, gate_scale=gate_scale, w_up=w_up, up_scale=up_scale)
+    q = torch.empty((M, N), dtype=_F8, device=dev)
+    scale = torch.empty(_act_scale_shape(M, N), dtype=torch.float32, device=dev)
+    L = lib()
+    need = L.miq_gated_fp8_workspace(M, N, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    with _on(dev):
+        _check(L.miq_gated_fp8(_ptr(x), _ptr(x_scale), _ptr(w_gate), _ptr(gate_scale), _ptr(w_up), _ptr(up_scale), M, N, K,
+                               _ACT_CODES[act], _ptr(q), _ptr(scale), _ptr(ws), need, _stream()))
+    return q, scale

@@ -1,0 +1,341 @@
+// Quantizers to block-scaled e4m3 and the root-mean-square norm that ends in one (gfx950; all three HBM-bound).
+//
+// Sixteen lanes (a DPP row) own a block of 128 columns, eight consecutive columns a lane: the block's maximum is four DPP
+// steps away, a 16-bit element row is read with one 16-byte load a lane and its codes leave as 8 bytes a lane, 128 bytes a
+// block.  Scales are block-major, [blocks, M]: the product reads one block of many rows at a time.
+#include "miq_fp8.h"
+
+namespace {
+
+using namespace miq;
+
+// ---- activations: 1 x 128 ------------------------------------------------------------------------------------------
+// A workgroup of 16 sixteen-lane groups takes ROWS rows x (16 / ROWS) * PASSES blocks.
+constexpr int kQuantPasses = 4;
+
+template <int DT, bool VEC, int ROWS>
+__global__ __launch_bounds__(256) void quantize_blocks_kernel(const void* __restrict__ x, int64_t M, int64_t K, int64_t kblocks,
+                                                              int64_t col_groups, uint8_t* __restrict__ q,
+                                                              float* __restrict__ scale) {
+    constexpr int kAcross = 16 / ROWS;   // blocks of one row that a pass covers
+    const int grp = threadIdx.x >> 4, lane = threadIdx.x & 15;
+    const int64_t m = (blockIdx.x / col_groups) * ROWS + grp / kAcross;
+    const int64_t kb0 = (blockIdx.x % col_groups) * (kAcross * kQuantPasses) + grp % kAcross;
+    float f[kQuantPasses][8];
+    int n[kQuantPasses];
+#pragma unroll
+    for (int p = 0; p < kQuantPasses; ++p) {
+        const int64_t k = (kb0 + p * kAcross) * kBlockK + lane * 8;
+        n[p] = m < M && k < K ? static_cast<int>(K - k < 8 ? K - k : 8) : 0;
+        load8<DT, VEC>(x, m * K + k, n[p], f[p]);
+    }
+#pragma unroll
+    for (int p = 0; p < kQuantPasses; ++p) {
+        const int64_t kb = kb0 + p * kAcross;
+        uint32_t c[2];
+        const float s = quantize8_in_row(f[p], c);
+        store8_codes<VEC>(q, m * K + kb * kBlockK + lane * 8, n[p], c);
+        if (lane == 0 && m < M && kb < kblocks) scale[kb * M + m] = s;
+    }
+}
+
+// ---- weights: 128 x 128 --------------------------------------------------------------------------------------------
+// One workgroup a block: a thread holds eight columns of eight rows (64 values) in registers.
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void quantize_weight_kernel(const void* __restrict__ w, int64_t N, int64_t K, int64_t kblocks,
+                                                              uint8_t* __restrict__ q, float* __restrict__ scale) {
+    __shared__ uint32_t tops[2][4];
+    const int grp = threadIdx.x >> 4, lane = threadIdx.x & 15, wave = threadIdx.x >> 6;
+    const int64_t nb = blockIdx.x / kblocks, kb = blockIdx.x % kblocks;
+    const int64_t k = kb * kBlockK + lane * 8;
+    float f[8][8];
+    int n[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        const int64_t row = nb * 128 + r * 16 + grp;
+        n[r] = row < N && k < K ? static_cast<int>(K - k < 8 ? K - k : 8) : 0;
+        load8<DT, VEC>(w, row * K + k, n[r], f[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t b = magnitude_bits(f[r][i]);
+            top = b > top ? b : top;
+        }
+    auto over_workgroup = [&](uint32_t v, int slot) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint32_t other = __shfl_xor(v, o, 64);
+            v = other > v ? other : v;
+        }
+        if ((threadIdx.x & 63) == 0) tops[slot][wave] = v;
+        __syncthreads();
+        uint32_t t = tops[slot][0];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) t = tops[slot][i] > t ? tops[slot][i] : t;
+        return t;
+    };
+    top = over_workgroup(top, 0);
+    const bool spoiled = top >= kInfBits;   // the same in every thread of the workgroup
+    if (spoiled) {
+        top = 0;
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t b = finite_magnitude_bits(f[r][i]);
+                top = b > top ? b : top;
+            }
+        top = over_workgroup(top, 1);
+    }
+    const BlockScale s = block_scale(top);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        uint32_t c[2];
+        codes8(f[r], s.inv, spoiled, c);
+        store8_codes<VEC>(q, (nb * 128 + r * 16 + grp) * K + k, n[r], c);
+    }
+    if (threadIdx.x == 0) scale[nb * kblocks + kb] = s.scale;
+}
+
+// ---- root-mean-square norm -----------------------------------------------------------------------------------------
+// h = x + residual (rounded to the type it is stored in, so that the norm is the norm of the stored row), y = (h / rms) * g,
+// then y in blocks as above.  TPR threads a row; a row of at most TPR * 8 * VPT columns stays in registers between the sum
+// of squares and the codes (VPT > 0); a longer one is read twice (VPT = 0).
+template <int DT>
+__device__ __forceinline__ float round_to(float v) {
+    if constexpr (DT == MIQ_BF16) return static_cast<float>(static_cast<__bf16>(v));
+    if constexpr (DT == MIQ_F16) return static_cast<float>(static_cast<_Float16>(v));
+    return v;
+}
+
+template <int DT, bool VEC>
+__device__ __forceinline__ void store8(void* base, int64_t index, int n, const float (&f)[8]) {
+    if constexpr (DT == MIQ_F32) {
+        float* p = static_cast<float*>(base) + index;
+        if constexpr (VEC) {
+            if (n > 0) {
+                typedef float f32x4 __attribute__((ext_vector_type(4)));
+                reinterpret_cast<f32x4*>(p)[0] = f32x4{f[0], f[1], f[2], f[3]};
+                reinterpret_cast<f32x4*>(p)[1] = f32x4{f[4], f[5], f[6], f[7]};
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < n) p[i] = f[i];
+        }
+    } else {
+        uint16_t* p = static_cast<uint16_t*>(base) + index;
+        uint16_t h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (DT == MIQ_BF16) h[i] = __builtin_bit_cast(uint16_t, static_cast<__bf16>(f[i]));
+            else h[i] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(f[i]));
+        }
+        if constexpr (VEC) {
+            if (n > 0) {
+                u32x4 v;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = h[2 * i] | (static_cast<uint32_t>(h[2 * i + 1]) << 16);
+                *reinterpret_cast<u32x4*>(p) = v;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < n) p[i] = h[i];
+        }
+    }
+}
+
+struct NormArgs {
+    const void* x;
+    const void* residual;   // or null
+    const void* g;
+    int g_f32;              // g is fp32, else of x's type
+    int64_t M, K, kblocks;
+    float eps;
+    void* sum;              // x + residual, written when there is a residual
+    uint8_t* q;
+    float* scale;
+};
+
+template <int DT, bool VEC, int TPR, int VPT>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(NormArgs a) {
+    constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR, kWaves = TPR / 64;
+    constexpr int kKeep = VPT > 0 ? VPT : 1;
+    __shared__ float part[kThreads / 64];
+    const int t = threadIdx.x % TPR;
+    const int64_t m = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
+    const bool live = m < a.M;
+    const int64_t row = m * a.K;
+    const int64_t vecs = (a.kblocks * kBlockK) / 8;            // whole blocks: all 16 lanes of a block take part
+    const int64_t rounds = (vecs + TPR - 1) / TPR;
+    auto count = [&](int64_t k) { return live && k < a.K ? static_cast<int>(a.K - k < 8 ? a.K - k : 8) : 0; };
+    auto load_h = [&](int64_t k, int n, float (&h)[8], bool write) {
+        load8<DT, VEC>(a.x, row + k, n, h);
+        if (a.residual) {
+            float r[8];
+            load8<DT, VEC>(a.residual, row + k, n, r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[i] = round_to<DT>(__fadd_rn(h[i], r[i]));
+            if (write) store8<DT, VEC>(a.sum, row + k, n, h);
+        }
+    };
+    float h[kKeep][8];
+    float ss = 0.0f;
+    if constexpr (VPT > 0) {
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int64_t k = (static_cast<int64_t>(v) * TPR + t) * 8;
+            load_h(k, count(k), h[v], true);
+        }
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            float s8 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s8 = __fadd_rn(s8, __fmul_rn(h[v][i], h[v][i]));
+            ss += s8;
+        }
+    } else {
+        for (int64_t v = 0; v < rounds; ++v) {
+            const int64_t k = (v * TPR + t) * 8;
+            load_h(k, count(k), h[0], true);
+            float s8 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s8 = __fadd_rn(s8, __fmul_rn(h[0][i], h[0][i]));
+            ss += s8;
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    if constexpr (kWaves > 1) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ss;
+        __syncthreads();
+        ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) ss += part[i];
+    }
+    const float inv_rms = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(a.K)), a.eps)));
+    auto finish = [&](int64_t k, int n, float (&hv)[8]) {
+        float g[8];
+        if (DT == MIQ_F32 || a.g_f32) load8<MIQ_F32, VEC>(a.g, k, k < a.K ? (a.K - k < 8 ? a.K - k : 8) : 0, g);
+        else load8<DT, VEC>(a.g, k, k < a.K ? (a.K - k < 8 ? a.K - k : 8) : 0, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) hv[i] = __fmul_rn(__fmul_rn(hv[i], inv_rms), g[i]);
+        uint32_t c[2];
+        const float s = quantize8_in_row(hv, c);
+        store8_codes<VEC>(a.q, row + k, n, c);
+        if ((threadIdx.x & 15) == 0 && n > 0) a.scale[(k / kBlockK) * a.M + m] = s;
+    };
+    if constexpr (VPT > 0) {
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int64_t k = (static_cast<int64_t>(v) * TPR + t) * 8;
+            finish(k, count(k), h[v]);
+        }
+    } else {
+        for (int64_t v = 0; v < rounds; ++v) {
+            const int64_t k = (v * TPR + t) * 8;
+            load_h(k, count(k), h[0], false);
+            finish(k, count(k), h[0]);
+        }
+    }
+}
+
+bool float_code(int dt) { return dt == MIQ_F32 || dt == MIQ_F16 || dt == MIQ_BF16; }
+int elem_size(int dt) { return dt == MIQ_F32 ? 4 : 2; }
+
+template <typename F>
+int for_dtype(int dt, F&& f) {
+    if (dt == MIQ_F32) return f(std::integral_constant<int, MIQ_F32>{});
+    if (dt == MIQ_F16) return f(std::integral_constant<int, MIQ_F16>{});
+    return f(std::integral_constant<int, MIQ_BF16>{});
+}
+
+constexpr int64_t kMaxGrid = (1ll << 24) - 1;   // 256 threads each: a launch holds less than 2^32 threads
+
+}  // namespace
+
+extern "C" int miq_quantize_blocks_fp8(const void* x, int x_dtype, int64_t M, int64_t K, uint8_t* q, float* scale,
+                                       void* stream) {
+    MIQ_REQUIRE(M >= 0 && K >= 0, MIQ_EINVAL, "miq_quantize_blocks_fp8: negative size (M=%lld K=%lld)", (long long)M, (long long)K);
+    MIQ_REQUIRE(float_code(x_dtype), MIQ_EINVAL, "miq_quantize_blocks_fp8: unknown x_dtype %d", x_dtype);
+    if (M == 0 || K == 0) return MIQ_OK;
+    MIQ_REQUIRE(all_below_2_31({M, K}), MIQ_ERANGE, "miq_quantize_blocks_fp8: a dimension at or beyond 2^31");
+    MIQ_REQUIRE(x && q && scale, MIQ_EINVAL, "miq_quantize_blocks_fp8: null pointer");
+    MIQ_REQUIRE(aligned(x, elem_size(x_dtype)) && aligned(scale, 4), MIQ_EALIGN, "miq_quantize_blocks_fp8: misaligned pointer");
+    const bool vec = K % 8 == 0 && aligned(x, 16) && aligned(q, 8);
+    const int64_t kblocks = ceil_div(K, kBlockK);
+    const bool tall = M >= 16;
+    const int64_t col_groups = ceil_div(kblocks, (tall ? 1 : 16) * kQuantPasses);
+    const int64_t grid = (tall ? ceil_div(M, 16) : M) * col_groups;
+    MIQ_REQUIRE(grid <= kMaxGrid, MIQ_ERANGE, "miq_quantize_blocks_fp8: too many blocks");
+    return for_dtype(x_dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        auto go = [&](auto v, auto rows) {
+            quantize_blocks_kernel<DT, decltype(v)::value, decltype(rows)::value>
+                <<<static_cast<unsigned>(grid), 256, 0, as_stream(stream)>>>(x, M, K, kblocks, col_groups, q, scale);
+        };
+        using R16 = std::integral_constant<int, 16>;
+        using R1 = std::integral_constant<int, 1>;
+        if (vec) tall ? go(std::true_type{}, R16{}) : go(std::true_type{}, R1{});
+        else tall ? go(std::false_type{}, R16{}) : go(std::false_type{}, R1{});
+        return check_launch("quantize_blocks_kernel");
+    });
+}
+
+extern "C" int miq_quantize_weight_fp8(const void* w, int w_dtype, int64_t N, int64_t K, uint8_t* q, float* scale,
+                                       void* stream) {
+    MIQ_REQUIRE(N >= 0 && K >= 0, MIQ_EINVAL, "miq_quantize_weight_fp8: negative size (N=%lld K=%lld)", (long long)N, (long long)K);
+    MIQ_REQUIRE(float_code(w_dtype), MIQ_EINVAL, "miq_quantize_weight_fp8: unknown w_dtype %d", w_dtype);
+    if (N == 0 || K == 0) return MIQ_OK;
+    MIQ_REQUIRE(all_below_2_31({N, K}), MIQ_ERANGE, "miq_quantize_weight_fp8: a dimension at or beyond 2^31");
+    MIQ_REQUIRE(w && q && scale, MIQ_EINVAL, "miq_quantize_weight_fp8: null pointer");
+    MIQ_REQUIRE(aligned(w, elem_size(w_dtype)) && aligned(scale, 4), MIQ_EALIGN, "miq_quantize_weight_fp8: misaligned pointer");
+    const bool vec = K % 8 == 0 && aligned(w, 16) && aligned(q, 8);
+    const int64_t kblocks = ceil_div(K, kBlockK), grid = ceil_div(N, 128) * kblocks;
+    MIQ_REQUIRE(grid <= kMaxGrid, MIQ_ERANGE, "miq_quantize_weight_fp8: too many blocks");
+    return for_dtype(w_dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (vec) quantize_weight_kernel<DT, true><<<static_cast<unsigned>(grid), 256, 0, as_stream(stream)>>>(w, N, K, kblocks, q, scale);
+        else quantize_weight_kernel<DT, false><<<static_cast<unsigned>(grid), 256, 0, as_stream(stream)>>>(w, N, K, kblocks, q, scale);
+        return check_launch("quantize_weight_kernel");
+    });
+}
+
+extern "C" int miq_rms_norm_fp8(const void* x, const void* residual, const void* weight, int dtype, int weight_dtype, int64_t M,
+                                int64_t K, float eps, void* sum, uint8_t* q, float* scale, void* stream) {
+    MIQ_REQUIRE(M >= 0 && K >= 0, MIQ_EINVAL, "miq_rms_norm_fp8: negative size (M=%lld K=%lld)", (long long)M, (long long)K);
+    MIQ_REQUIRE(float_code(dtype), MIQ_EINVAL, "miq_rms_norm_fp8: unknown dtype %d", dtype);
+    MIQ_REQUIRE(weight_dtype == dtype || weight_dtype == MIQ_F32, MIQ_EINVAL,
+                "miq_rms_norm_fp8: weight_dtype must be dtype or MIQ_F32 (got %d)", weight_dtype);
+    MIQ_REQUIRE(eps >= 0.0f && eps < __builtin_inff(), MIQ_EINVAL, "miq_rms_norm_fp8: eps must be finite and not negative");
+    if (M == 0 || K == 0) return MIQ_OK;
+    MIQ_REQUIRE(all_below_2_31({M, K}), MIQ_ERANGE, "miq_rms_norm_fp8: a dimension at or beyond 2^31");
+    MIQ_REQUIRE(x && weight && q && scale, MIQ_EINVAL, "miq_rms_norm_fp8: null pointer");
+    MIQ_REQUIRE((residual == nullptr) == (sum == nullptr), MIQ_EINVAL, "miq_rms_norm_fp8: residual and sum come together");
+    const int es = elem_size(dtype);
+    MIQ_REQUIRE(aligned(x, es) && aligned(residual, es) && aligned(sum, es) && aligned(weight, elem_size(weight_dtype)) && aligned(scale, 4),
+                MIQ_EALIGN, "miq_rms_norm_fp8: misaligned pointer");
+    const bool vec = K % 8 == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(sum, 16) && aligned(weight, 16) && aligned(q, 8);
+    NormArgs a{x, residual, weight, weight_dtype == MIQ_F32, M, K, ceil_div(K, kBlockK), eps, sum, q, scale};
+    const int64_t cols = a.kblocks * kBlockK;
+    MIQ_REQUIRE(M * (cols <= 256 * 32 ? 256 : 1024) < (1ll << 32), MIQ_ERANGE, "miq_rms_norm_fp8: too many rows");
+    return for_dtype(dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        auto go = [&](auto v) {
+            constexpr bool V = decltype(v)::value;
+            const unsigned grid = static_cast<unsigned>(M);
+            if (cols <= 256 * 8) rms_norm_kernel<DT, V, 256, 1><<<grid, 256, 0, as_stream(stream)>>>(a);
+            else if (cols <= 256 * 16) rms_norm_kernel<DT, V, 256, 2><<<grid, 256, 0, as_stream(stream)>>>(a);
+            else if (cols <= 256 * 32) rms_norm_kernel<DT, V, 256, 4><<<grid, 256, 0, as_stream(stream)>>>(a);
+            else if (cols <= 1024 * 16) rms_norm_kernel<DT, V, 1024, 2><<<grid, 1024, 0, as_stream(stream)>>>(a);
+            else rms_norm_kernel<DT, V, 1024, 0><<<grid, 1024, 0, as_stream(stream)>>>(a);
+        };
+        if (vec) go(std::true_type{});
+        else go(std::false_type{});
+        return check_launch("rms_norm_kernel");
+    });
+}

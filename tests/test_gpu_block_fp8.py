@@ -1,0 +1,360 @@
+"""Block-scaled 8-bit floating point operators on the GPU against plain 64-bit forms (fp8_reference.py)."""
+import math
+
+import pytest
+import torch
+
+import fp8_reference as R
+
+pytestmark = pytest.mark.gpu
+FLOATS = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def rand(m, k, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g) * torch.exp(torch.randn(m, 1, generator=g))
+    x[:, torch.rand(k, generator=g) < 0.02] *= 30.0
+    return x.to(dtype)
+
+
+def codes(m, k, seed, weight=False):
+    """Codes and scales by the reference, so that a product's test does not rest on the quantizer's kernel."""
+    x = rand(m, k, torch.float32, seed)
+    q, s = (R.quantize_weight if weight else R.quantize_rows)(x)
+    return q.to(torch.float32).to(torch.float8_e4m3fn), s
+
+
+def same_codes(q, ref):
+    got = q.cpu().to(torch.float32).double()
+    nan = torch.isnan(ref)
+    assert torch.equal(torch.isnan(got), nan)
+    assert torch.equal(got[~nan], ref[~nan])
+
+
+# ---- quantizers: the documented fp32 arithmetic, bit for bit ---------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 128), (3, 7), (1, 4096), (2, 1000), (15, 129), (16, 384), (17, 2056), (33, 515), (130, 8), (5, 20000)])
+def test_quantize_blocks(dtype, m, k):
+    from quantization_amd import block_fp8 as F
+    x = rand(m, k, dtype, 7 * m + k)
+    q, s = F.quantize_blocks_fp8(x.cuda())
+    rq, rs = R.quantize_rows(x)
+    assert q.dtype == torch.float8_e4m3fn and q.shape == x.shape
+    assert torch.equal(s.cpu(), rs)
+    same_codes(q, rq)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("n,k", [(1, 1), (128, 128), (127, 129), (129, 127), (300, 1000), (64, 16), (257, 512), (5, 4100)])
+def test_quantize_weight(dtype, n, k):
+    from quantization_amd import block_fp8 as F
+    w = rand(n, k, dtype, n + 3 * k)
+    q, s = F.quantize_weight_fp8(w.cuda())
+    rq, rs = R.quantize_weight(w)
+    assert torch.equal(s.cpu(), rs)
+    same_codes(q, rq)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("k", [384, 300])
+def test_quantize_extremes(dtype, k):
+    """Zero rows, the type's smallest and largest values, infinities and NaN: the last two become NaN codes and leave the
+    other codes of their block as they would be without them."""
+    from quantization_amd import block_fp8 as F
+    x = rand(40, k, dtype, 5)
+    info = torch.finfo(dtype)
+    x[0] = 0
+    x[1] = info.tiny
+    x[2] = info.smallest_normal * torch.randn(k, generator=torch.Generator().manual_seed(1)).to(dtype)
+    x[3] = info.min
+    x[4, ::2] = info.max
+    x[5, 3] = math.inf
+    x[6, 200] = -math.inf
+    x[7, 130] = math.nan
+    x[8] = math.nan
+    x[9, :128] = math.inf
+    x[10] = -0.0
+    x[11, 5], x[11, 6], x[11, 7] = math.nan, math.inf, info.max
+    q, s = F.quantize_blocks_fp8(x.cuda())
+    rq, rs = R.quantize_rows(x)
+    assert torch.equal(s.cpu(), rs) and bool((s > 0).all()) and bool(torch.isfinite(s).all())
+    same_codes(q, rq)
+    q, s = F.quantize_weight_fp8(x.cuda())
+    rq, rs = R.quantize_weight(x)
+    assert torch.equal(s.cpu(), rs)
+    same_codes(q, rq)
+
+
+def test_quantize_unaligned_storage():
+    """A dense matrix that starts at an odd element of its storage, and one behind it that must stay as it was."""
+    from quantization_amd import block_fp8 as F
+    for dtype in FLOATS:
+        buf = rand(1, 20 * 256 + 3, dtype, 9)[0].cuda()
+        x = buf[1:1 + 20 * 256].view(20, 256)
+        q, s = F.quantize_blocks_fp8(x)
+        rq, rs = R.quantize_rows(x)
+        assert torch.equal(s.cpu(), rs)
+        same_codes(q, rq)
+        q, s = F.quantize_weight_fp8(x)
+        rq, rs = R.quantize_weight(x)
+        assert torch.equal(s.cpu(), rs)
+        same_codes(q, rq)
+
+
+# ---- norm ------------------------------------------------------------------------------------------------------------
+
+def norm_reference(x, g, eps, residual):
+    """(y in float64, bound on its error in fp32, the stored sum).  Each square is rounded and the sum of k of them takes at
+    most 8 + ceil(k / 2048) + 22 additions on the longest path (eight values a thread, the thread's vectors, six shuffles and
+    sixteen waves); the quotient, the addition, the root, its inverse and two products follow."""
+    total = None
+    h = x.cpu()
+    if residual is not None:
+        total = (x.cpu().double() + residual.cpu().double()).to(x.dtype) if x.dtype != torch.float32 else x.cpu() + residual.cpu()
+        h = total
+    h = h.double()
+    k = h.shape[1]
+    y = h / torch.sqrt(h.square().sum(dim=1, keepdim=True) / k + eps) * g.cpu().double()
+    steps = 1 + 8 + -(-k // 2048) + 22
+    return y, (0.5 * steps + 8) * 2.0 ** -23 * y.abs(), total
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 4096), (2, 100), (3, 129), (5, 2048), (4, 2056), (3, 5000), (2, 8192), (2, 8200), (3, 9001), (1, 16384), (2, 16392), (2, 40001)])
+def test_rms_norm(dtype, residual, m, k):
+    from quantization_amd import block_fp8 as F
+    x = rand(m, k, dtype, k)
+    r = rand(m, k, dtype, k + 1) if residual else None
+    for gt in {dtype, torch.float32}:
+        g = (1 + 0.2 * torch.randn(k, generator=torch.Generator().manual_seed(k))).to(gt)
+        got = F.rms_norm_fp8(x.cuda(), g.cuda(), 1e-5, residual=None if r is None else r.cuda())
+        y, dy, total = norm_reference(x, g, 1e-5, r)
+        R.check_codes_of(got[0], got[1], y, dy)
+        if residual:
+            assert torch.equal(got[2].cpu(), total)
+        else:
+            assert len(got) == 2
+
+
+def test_rms_norm_empty_mask_rows_and_spoiled_rows():
+    """Rows of zeros (nothing to norm: codes 0), a row with a NaN (all NaN), others untouched by it."""
+    from quantization_amd import block_fp8 as F
+    x = rand(6, 640, torch.bfloat16, 3)
+    x[0] = 0
+    x[2, 17] = math.nan
+    g = torch.ones(640, dtype=torch.bfloat16)
+    q, s = F.rms_norm_fp8(x.cuda(), g.cuda(), 1e-6)
+    assert not bool(q[0].float().any()) and bool((s[:, 0] > 0).all())
+    assert bool(torch.isnan(q[2].float()).all())
+    keep = [0, 1, 3, 4, 5]
+    y, dy, _ = norm_reference(x[keep], g, 1e-6, None)
+    R.check_codes_of(q[keep], s[:, keep], y, dy)
+
+
+# ---- products ----------------------------------------------------------------------------------------------------------
+
+PRODUCTS = [(1, 1, 1), (1, 64, 16), (1, 130, 4096), (2, 129, 100), (7, 300, 1000), (15, 257, 1024), (16, 128, 128), (17, 640, 2064),
+            (33, 100, 129), (64, 513, 384), (65, 256, 4100), (100, 96, 400), (129, 384, 1040), (257, 260, 256), (300, 700, 136),
+            (70, 1, 300), (520, 270, 640)]
+
+
+@pytest.mark.parametrize("out", FLOATS)
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_linear(out, m, n, k):
+    from quantization_amd import block_fp8 as F
+    xq, xs = codes(m, k, m + n + k)
+    wq, ws = codes(n, k, m * n + k, weight=True)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(n)) if (m + n) % 2 else None
+    y = F.linear_fp8(xq.cuda(), xs.cuda(), wq.cuda(), ws.cuda(), None if bias is None else bias.cuda(), out)
+    assert y.shape == (m, n) and y.dtype == out
+    ref, mag = R.product(xq, xs, wq, ws)
+    err = R.product_error(mag, k)
+    if bias is not None:
+        ref = ref + bias.double()
+        err = err + 2.0 ** -24 * (ref.abs() + err)
+    half = torch.finfo(out).eps / 2
+    fits = ref.abs() < torch.finfo(out).max * 0.99
+    off = (y.cpu().double() - ref).abs()
+    tol = err + half * (ref.abs() + err) + torch.finfo(out).smallest_normal * torch.finfo(out).eps
+    assert bool((off <= tol)[fits].all()), float((off / tol)[fits].max())
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_gated(act, m, n, k):
+    from quantization_amd import block_fp8 as F
+    xq, xs = codes(m, k, m + n)
+    gq, gs = codes(n, k, n + k, weight=True)
+    uq, us = codes(n, k, n + k + 1, weight=True)
+    gs = gs * 0.05   # gates of order one: the bend of the activation
+    q, s = F.gated_linear_fp8(xq.cuda(), xs.cuda(), gq.cuda(), gs.cuda(), uq.cuda(), us.cuda(), act)
+    assert q.shape == (m, n) and q.dtype == torch.float8_e4m3fn
+    y, dy = gated_reference(xq, xs, gq, gs, uq, us, act)
+    R.check_codes_of(q, s, y, dy)
+
+
+def gated_reference(xq, xs, gq, gs, uq, us, act):
+    """(act(g) * u, its bound): |act'| is at most 1.13 for both, |act(g)| at most |g|; the activation's own steps (exponential
+    or error function, sum, quotient, products) are within 8 units relative to |g|, which bounds it."""
+    k = xq.shape[1]
+    g, gmag = R.product(xq, xs, gq, gs)
+    u, umag = R.product(xq, xs, uq, us)
+    dg, du = R.product_error(gmag, k), R.product_error(umag, k)
+    a = R.act(g, act)
+    da = 1.13 * dg + 8 * 2.0 ** -23 * g.abs()
+    y = a * u
+    return y, da * (u.abs() + du) + a.abs() * du + 2.0 ** -23 * y.abs()
+
+
+def test_products_of_nan_codes_and_zero_rows():
+    """A NaN code spoils its own row (activation) or column (weight) of the product only; a row of zero codes gives the bias."""
+    from quantization_amd import block_fp8 as F
+    for m, k in ((5, 272), (40, 272), (200, 100)):
+        xq, xs = codes(m, k, 1)
+        wq, ws = codes(150, k, 2, weight=True)
+        x = xq.float()
+        x[3, k - 1] = math.nan
+        x[1] = 0
+        w = wq.float()
+        w[149, 0] = math.nan
+        xq, wq = x.to(torch.float8_e4m3fn), w.to(torch.float8_e4m3fn)
+        bias = torch.randn(150, generator=torch.Generator().manual_seed(4))
+        y = F.linear_fp8(xq.cuda(), xs.cuda(), wq.cuda(), ws.cuda(), bias.cuda(), torch.float32).cpu()
+        nan = torch.zeros(m, 150, dtype=torch.bool)
+        nan[3], nan[:, 149] = True, True
+        assert torch.equal(torch.isnan(y), nan)
+        assert torch.equal(y[1, :149], bias[:149])
+        q, s = F.gated_linear_fp8(xq.cuda(), xs.cuda(), wq.cuda(), ws.cuda(), wq.cuda(), ws.cuda())
+        assert torch.equal(torch.isnan(q.float().cpu()), nan)
+        assert bool(torch.isfinite(s).all()) and not bool(q[1, :149].float().any())
+
+
+def test_unaligned_codes():
+    """Dense code matrices that start at an odd byte."""
+    from quantization_amd import block_fp8 as F
+    for m in (3, 40, 150):
+        xq, xs = codes(m, 256, 11)
+        wq, ws = codes(200, 256, 12, weight=True)
+        xb, wb = torch.zeros(m * 256 + 1, dtype=torch.uint8, device="cuda"), torch.zeros(200 * 256 + 5, dtype=torch.uint8, device="cuda")
+        xb[1:] = xq.view(torch.uint8).reshape(-1).cuda()
+        wb[5:] = wq.view(torch.uint8).reshape(-1).cuda()
+        x1, w1 = xb[1:].view(torch.float8_e4m3fn).view(m, 256), wb[5:].view(torch.float8_e4m3fn).view(200, 256)
+        a = F.linear_fp8(x1, xs.cuda(), w1, ws.cuda(), None, torch.float32).cpu().double()
+        ref, mag = R.product(xq, xs, wq, ws)
+        assert bool(((a - ref).abs() <= R.product_error(mag, 256) + 2.0 ** -24 * ref.abs()).all())
+
+
+def test_empty_sizes():
+    from quantization_amd import block_fp8 as F
+    dev = "cuda"
+    q, s = F.quantize_blocks_fp8(torch.zeros(0, 256, device=dev))
+    assert q.shape == (0, 256) and s.shape == (2, 0)
+    w, ws = F.quantize_weight_fp8(torch.randn(130, 256, device=dev))
+    assert F.linear_fp8(q, s, w, ws).shape == (0, 130)
+    h, hs = F.gated_linear_fp8(q, s, w, ws, w, ws)
+    assert h.shape == (0, 130) and hs.shape == (2, 0)
+    q, s = F.rms_norm_fp8(torch.zeros(0, 256, device=dev), torch.ones(256, device=dev))
+    assert q.shape == (0, 256)
+    x0, s0 = F.quantize_blocks_fp8(torch.zeros(3, 0, device=dev))
+    w0, ws0 = F.quantize_weight_fp8(torch.zeros(5, 0, device=dev))
+    y = F.linear_fp8(x0, s0, w0, ws0, torch.arange(5.0, device=dev), torch.float32)
+    assert torch.equal(y, torch.arange(5.0, device=dev).expand(3, 5))
+
+
+# ---- together ------------------------------------------------------------------------------------------------------------
+
+def block_weights(k, n, seed, dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(seed)
+    mats = [(torch.randn(a, b, generator=g) / math.sqrt(b)).to(dtype).cuda() for a, b in ((n, k), (n, k), (k, n))]
+    return mats, (1 + 0.1 * torch.randn(k, generator=g)).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("lead,k,n", [((1,), 512, 1408), ((3, 7), 520, 900), ((2, 70), 256, 640), ((300,), 384, 1000)])
+def test_feed_forward_block(lead, k, n):
+    """norm with residual -> gate and up -> down, each stage against the 64-bit form of what it was given."""
+    from quantization_amd import block_fp8 as F
+    (wg, wu, wd), gain = block_weights(k, n, 5)
+    g8, u8, d8 = (F.quantize_weight_fp8(w) for w in (wg, wu, wd))
+    m = math.prod(lead)
+    x, r = (rand(m, k, torch.bfloat16, s).view(*lead, k).cuda() for s in (1, 2))
+    q, s, h = F.rms_norm_fp8(x, gain, 1e-5, residual=r)
+    assert q.shape == x.shape and h.shape == x.shape
+    y, dy, total = norm_reference(x.view(m, k), gain, 1e-5, r.view(m, k))
+    R.check_codes_of(q.view(m, k), s, y, dy)
+    assert torch.equal(h.cpu().view(m, k), total)
+    hq, hs = F.gated_linear_fp8(q, s, *g8, *u8)
+    assert hq.shape == (*lead, n)
+    y, dy = gated_reference(q.view(m, k), s, *g8, *u8, "silu")
+    R.check_codes_of(hq.view(m, n), hs, y, dy)
+    out = F.linear_fp8(hq, hs, *d8)
+    assert out.shape == x.shape
+    ref, mag = R.product(hq.view(m, n), hs, *d8)
+    err = R.product_error(mag, n)
+    assert bool(((out.cpu().double().view(m, k) - ref).abs() <= err + 2.0 ** -8 * (ref.abs() + err) + 1e-38).all())
+
+
+def test_captured_and_replayed():
+    """The block captured into a HIP graph (two of them, of different sizes, replayed in turn with eager calls between)
+    gives the eager results on new inputs."""
+    from quantization_amd import block_fp8 as F
+    (wg, wu, wd), gain = block_weights(512, 1152, 8)
+    g8, u8, d8 = (F.quantize_weight_fp8(w) for w in (wg, wu, wd))
+
+    def block(x, r):
+        q, s, h = F.rms_norm_fp8(x, gain, 1e-5, residual=r)
+        return F.linear_fp8(*F.gated_linear_fp8(q, s, *g8, *u8), *d8) + h
+
+    graphs = []
+    for m in (1, 48, 300):
+        x, r = torch.zeros(m, 512, dtype=torch.bfloat16, device="cuda"), torch.zeros(m, 512, dtype=torch.bfloat16, device="cuda")
+        block(x, r)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            block(x, r)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = block(x, r)
+        graphs.append((m, x, r, y, graph))
+    for step in range(4):
+        for m, x, r, y, graph in graphs:
+            x.copy_(rand(m, 512, torch.bfloat16, step))
+            r.copy_(rand(m, 512, torch.bfloat16, step + 50))
+            graph.replay()
+            want = block(x.clone(), r.clone())
+            torch.cuda.synchronize()
+            assert torch.equal(y, want)
+
+
+def test_two_streams():
+    """Two streams at once, each with its own tensors."""
+    from quantization_amd import block_fp8 as F
+    w8 = F.quantize_weight_fp8(rand(700, 4096, torch.bfloat16, 1).cuda())
+    xs = [rand(m, 4096, torch.bfloat16, m).cuda() for m in (1, 33)]
+    want = [F.linear_fp8(*F.quantize_blocks_fp8(x), *w8) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(5):
+        got = []
+        for x, st in zip(xs, streams):
+            with torch.cuda.stream(st):
+                got.append(F.linear_fp8(*F.quantize_blocks_fp8(x), *w8))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("m", [1, 16, 40, 300])
+def test_same_call_same_bits(m):
+    """No result depends on the order in which workgroups finish."""
+    from quantization_amd import block_fp8 as F
+    xq, xs = (t.cuda() for t in codes(m, 8192, 3))
+    w8 = F.quantize_weight_fp8(rand(512, 8192, torch.bfloat16, 1).cuda())
+    a, b = F.linear_fp8(xq, xs, *w8), F.gated_linear_fp8(xq, xs, *w8, *w8)
+    for _ in range(3):
+        assert torch.equal(F.linear_fp8(xq, xs, *w8), a)
+        c = F.gated_linear_fp8(xq, xs, *w8, *w8)
+        assert torch.equal(c[0].view(torch.uint8), b[0].view(torch.uint8)) and torch.equal(c[1], b[1])
