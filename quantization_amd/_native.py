@@ -790,124 +790,148 @@ def epilogue_channels_f32(y, bias, alpha, beta=0.0):
 
 
 # ---- block-scaled 8-bit floating point ------------------------------------------------------------------------------
+# A norm or a quantizer of one token runs for a few microseconds, less than a careless wrapper: these functions pass plain
+# integers to ctypes (no c_void_p objects), read the current stream as an integer, and look at each tensor once.
 
 _F8 = torch.float8_e4m3fn
 _FP8_OUT_CODES = _FLOAT_CODES
 _ACT_CODES = {"silu": MIQ_ACT_SILU, "gelu": MIQ_ACT_GELU}
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    lambda index: torch.cuda.current_stream(index).cuda_stream
 
 
-def _require_same_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise RuntimeError(f"{name} must be on {device} (got {t.device})")
+def _launch(fn, index, *args):
+    """fn(*args, the current stream of device `index`), with that device current."""
+    current = torch.cuda.current_device()
+    if current == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        torch.cuda.set_device(index)
+        try:
+            rc = fn(*args, _raw_stream(index))
+        finally:
+            torch.cuda.set_device(current)
+    if rc:
+        _check(rc)
 
 
-def _fp8_matrix(q, scale, name, scale_shape):
-    """Checks a matrix of codes and its scales; returns (rows, columns)."""
-    require_device(q, name)
-    require_device(scale, f"the scales of {name}")
-    if q.dtype != _F8 or q.dim() != 2:
-        raise RuntimeError(f"{name} must be a float8_e4m3fn matrix, got {tuple(q.shape)} {q.dtype}")
-    if scale.dtype != torch.float32 or tuple(scale.shape) != scale_shape(*q.shape):
-        raise RuntimeError(f"the scales of {name} {tuple(q.shape)} must be float32 {scale_shape(*q.shape)}, got {tuple(scale.shape)} {scale.dtype}")
-    return q.shape
-
-
-def _act_scale_shape(m, k):
-    return ((k + 127) // 128, m)
-
-
-def _weight_scale_shape(n, k):
-    return ((n + 127) // 128, (k + 127) // 128)
+def _require(t, index, name):
+    """t is dense and on GPU `index`."""
+    if t.get_device() != index:
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must be a CUDA tensor")
+        raise RuntimeError(f"{name} must be on cuda:{index} (got {t.device})")
+    if not t.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
 
 
 def _float_matrix(x, name):
+    """(rows, columns, type code, device index) of a dense float matrix on a GPU."""
     require_device(x, name)
-    if x.dtype not in _FLOAT_CODES or x.dim() != 2:
+    code = _FLOAT_CODES.get(x.dtype)
+    if code is None or x.dim() != 2:
         raise RuntimeError(f"{name} must be a float32, float16 or bfloat16 matrix, got {tuple(x.shape)} {x.dtype}")
-    return x.shape
+    return (*x.shape, code, x.get_device())
+
+
+def _codes_matrix(q, scale, index, name, weight):
+    """(rows, columns) of a dense matrix of codes whose scales are those of an activation or of a weight."""
+    _require(q, index, name)
+    _require(scale, index, f"the scales of {name}")
+    if q.dtype is not _F8 or q.dim() != 2:
+        raise RuntimeError(f"{name} must be a float8_e4m3fn matrix, got {tuple(q.shape)} {q.dtype}")
+    r, c = q.shape
+    want = ((r + 127) // 128, (c + 127) // 128) if weight else ((c + 127) // 128, r)
+    if scale.dtype is not torch.float32 or scale.shape != want:
+        raise RuntimeError(f"the scales of {name} {tuple(q.shape)} must be float32 {want}, got {tuple(scale.shape)} {scale.dtype}")
+    return r, c
+
+
+def _aligned16(t):
+    """t, or a copy of it where it starts at an address that is no multiple of 16 (a view into the middle of a storage)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def quantize_blocks_fp8(x):
     """x [M, K] float -> (codes float8_e4m3fn [M, K], scales fp32 [ceil(K / 128), M])."""
-    M, K = _float_matrix(x, "input")
-    q = torch.empty((M, K), dtype=_F8, device=x.device)
-    scale = torch.empty(_act_scale_shape(M, K), dtype=torch.float32, device=x.device)
-    with _on(x.device):
-        _check(lib().miq_quantize_blocks_fp8(_ptr(x), _FLOAT_CODES[x.dtype], M, K, _ptr(q), _ptr(scale), _stream()))
+    M, K, code, index = _float_matrix(x, "input")
+    q = torch.empty_like(x, dtype=_F8)
+    scale = x.new_empty(((K + 127) // 128, M), dtype=torch.float32)
+    _launch(lib().miq_quantize_blocks_fp8, index, x.data_ptr(), code, M, K, q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
 def quantize_weight_fp8(w):
     """w [N, K] float -> (codes float8_e4m3fn [N, K], scales fp32 [ceil(N / 128), ceil(K / 128)])."""
-    N, K = _float_matrix(w, "weight")
-    q = torch.empty((N, K), dtype=_F8, device=w.device)
-    scale = torch.empty(_weight_scale_shape(N, K), dtype=torch.float32, device=w.device)
-    with _on(w.device):
-        _check(lib().miq_quantize_weight_fp8(_ptr(w), _FLOAT_CODES[w.dtype], N, K, _ptr(q), _ptr(scale), _stream()))
+    N, K, code, index = _float_matrix(w, "weight")
+    q = torch.empty_like(w, dtype=_F8)
+    scale = w.new_empty(((N + 127) // 128, (K + 127) // 128), dtype=torch.float32)
+    _launch(lib().miq_quantize_weight_fp8, index, w.data_ptr(), code, N, K, q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
 def rms_norm_fp8(x, weight, eps, residual=None):
     """x [M, K] float -> (codes, scales, x + residual or None)."""
-    M, K = _float_matrix(x, "input")
-    require_device(weight, "weight")
-    if tuple(weight.shape) != (K,) or weight.dtype not in (x.dtype, torch.float32):
+    M, K, code, index = _float_matrix(x, "input")
+    _require(weight, index, "weight")
+    if weight.shape != (K,) or weight.dtype not in (x.dtype, torch.float32):
         raise RuntimeError(f"weight must be [{K}] of {x.dtype} or float32, got {tuple(weight.shape)} {weight.dtype}")
     total = None
     if residual is not None:
-        require_device(residual, "residual")
+        _require(residual, index, "residual")
         if residual.shape != x.shape or residual.dtype != x.dtype:
             raise RuntimeError(f"residual must be {tuple(x.shape)} {x.dtype}, got {tuple(residual.shape)} {residual.dtype}")
         total = torch.empty_like(x)
-    _require_same_device(x.device, weight=weight, residual=residual)
-    q = torch.empty((M, K), dtype=_F8, device=x.device)
-    scale = torch.empty(_act_scale_shape(M, K), dtype=torch.float32, device=x.device)
-    with _on(x.device):
-        _check(lib().miq_rms_norm_fp8(_ptr(x), _ptr(residual), _ptr(weight), _FLOAT_CODES[x.dtype], _FLOAT_CODES[weight.dtype], M, K,
-                                      eps, _ptr(total), _ptr(q), _ptr(scale), _stream()))
+    q = torch.empty_like(x, dtype=_F8)
+    scale = x.new_empty(((K + 127) // 128, M), dtype=torch.float32)
+    _launch(lib().miq_rms_norm_fp8, index, x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(),
+            code, _FLOAT_CODES[weight.dtype], M, K, eps, None if total is None else total.data_ptr(), q.data_ptr(), scale.data_ptr())
     return q, scale, total
 
 
 def gemm_fp8(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16):
     """Codes x [M, K] times codes w [N, K]^T, each with its block scales, plus bias -> [M, N] of out_dtype."""
-    M, K = _fp8_matrix(x, x_scale, "input", _act_scale_shape)
-    N, Kw = _fp8_matrix(w, w_scale, "weight", _weight_scale_shape)
+    if not x.is_cuda:
+        raise RuntimeError("input must be a CUDA tensor")
+    index = x.get_device()
+    M, K = _codes_matrix(x, x_scale, index, "input", False)
+    N, Kw = _codes_matrix(w, w_scale, index, "weight", True)
     if K != Kw:
         raise RuntimeError(f"input has {K} columns, weight {Kw}")
-    if out_dtype not in _FP8_OUT_CODES:
+    code = _FP8_OUT_CODES.get(out_dtype)
+    if code is None:
         raise RuntimeError(f"unsupported output dtype {out_dtype}")
-    dev = x.device
-    _require_same_device(dev, x_scale=x_scale, weight=w, w_scale=w_scale)
-    bias = _f32_vec(bias, N, "bias", dev)
-    out = torch.empty((M, N), dtype=out_dtype, device=dev)
+    x, w = _aligned16(x), _aligned16(w)
+    bias = _f32_vec(bias, N, "bias", x.device)
+    out = x.new_empty((M, N), dtype=out_dtype)
     L = lib()
     need = L.miq_gemm_fp8_workspace(M, N, K)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with _on(dev):
-        _check(L.miq_gemm_fp8(_ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), M, N, K, _ptr(bias), _ptr(out),
-                              _FP8_OUT_CODES[out_dtype], _ptr(ws), need, _stream()))
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    _launch(L.miq_gemm_fp8, index, x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), M, N, K,
+            None if bias is None else bias.data_ptr(), out.data_ptr(), code, None if ws is None else ws.data_ptr(), need)
     return out
 
 
 def gated_fp8(x, x_scale, w_gate, gate_scale, w_up, up_scale, act="silu"):
     """Codes of act(x . w_gate^T) * (x . w_up^T): (codes [M, N], scales [ceil(N / 128), M])."""
-    M, K = _fp8_matrix(x, x_scale, "input", _act_scale_shape)
-    N, Kg = _fp8_matrix(w_gate, gate_scale, "gate weight", _weight_scale_shape)
+    if not x.is_cuda:
+        raise RuntimeError("input must be a CUDA tensor")
+    index = x.get_device()
+    M, K = _codes_matrix(x, x_scale, index, "input", False)
+    N, Kg = _codes_matrix(w_gate, gate_scale, index, "gate weight", True)
     if K != Kg:
         raise RuntimeError(f"input has {K} columns, gate weight {Kg}")
-    if _fp8_matrix(w_up, up_scale, "up weight", _weight_scale_shape) != w_gate.shape:
+    if _codes_matrix(w_up, up_scale, index, "up weight", True) != (N, K):
         raise RuntimeError(f"gate weight is {tuple(w_gate.shape)}, up weight {tuple(w_up.shape)}")
-    if act not in _ACT_CODES:
+    code = _ACT_CODES.get(act)
+    if code is None:
         raise RuntimeError(f"unknown activation {act!r}: silu or gelu")
-    dev = x.device
-    _require_same_device(dev, x_scale=x_scale, w_gate=w_gate, gate_scale=gate_scale, w_up=w_up, up_scale=up_scale)
-    q = torch.empty((M, N), dtype=_F8, device=dev)
-    scale = torch.empty(_act_scale_shape(M, N), dtype=torch.float32, device=dev)
+    x, w_gate, w_up = _aligned16(x), _aligned16(w_gate), _aligned16(w_up)
+    q = x.new_empty((M, N))
+    scale = x_scale.new_empty(((N + 127) // 128, M))
     L = lib()
     need = L.miq_gated_fp8_workspace(M, N, K)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with _on(dev):
-        _check(L.miq_gated_fp8(_ptr(x), _ptr(x_scale), _ptr(w_gate), _ptr(gate_scale), _ptr(w_up), _ptr(up_scale), M, N, K,
-                               _ACT_CODES[act], _ptr(q), _ptr(scale), _ptr(ws), need, _stream()))
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    _launch(L.miq_gated_fp8, index, x.data_ptr(), x_scale.data_ptr(), w_gate.data_ptr(), gate_scale.data_ptr(), w_up.data_ptr(),
+            up_scale.data_ptr(), M, N, K, code, q.data_ptr(), scale.data_ptr(), None if ws is None else ws.data_ptr(), need)
     return q, scale

@@ -28,38 +28,32 @@ def _rows(x):
     return x.reshape(x.shape[:-1].numel(), x.shape[-1]).contiguous()
 
 
-@torch.no_grad()
 def quantize_blocks_fp8(x):
     """x [..., K] float32, float16 or bfloat16 -> (codes [..., K], scales [ceil(K / 128), M])."""
-    _native.require_device(x, "input")
     q, scale = _native.quantize_blocks_fp8(_rows(x))
-    return q.view(x.shape), scale
+    return q if x.dim() == 2 else q.view(x.shape), scale
 
 
-@torch.no_grad()
 def quantize_weight_fp8(w):
     """w [N, K] -> (codes [N, K], scales [ceil(N / 128), ceil(K / 128)]); once, when a layer is built."""
     return _native.quantize_weight_fp8(w)
 
 
-@torch.no_grad()
 def rms_norm_fp8(x, weight, eps=1e-6, residual=None):
     """The codes of h / rms(h) * weight, with h = x (returns codes, scales) or, with a residual, h = x + residual rounded to
     x's type (returns codes, scales, h).  weight: [K] of x's type or float32."""
     q, scale, total = _native.rms_norm_fp8(_rows(x), weight, eps, None if residual is None else _rows(residual))
-    if residual is None:
-        return q.view(x.shape), scale
-    return q.view(x.shape), scale, total.view(x.shape)
+    if x.dim() != 2:
+        q, total = q.view(x.shape), None if total is None else total.view(x.shape)
+    return (q, scale) if residual is None else (q, scale, total)
 
 
-@torch.no_grad()
 def linear_fp8(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16):
     """x [..., K] codes with their scales, times w [N, K] codes with theirs, plus bias [N] -> [..., N] of out_dtype."""
     y = _native.gemm_fp8(_rows(x), x_scale, w, w_scale, bias, out_dtype)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[-1])
 
 
-@torch.no_grad()
 def gated_linear_fp8(x, x_scale, w_gate, gate_scale, w_up, up_scale, act="silu"):
     """The codes of act(x . w_gate^T) * (x . w_up^T): (codes [..., N], scales [ceil(N / 128), M]).  act: "silu" or "gelu"."""
     q, scale = _native.gated_fp8(_rows(x), x_scale, w_gate, gate_scale, w_up, up_scale, act)

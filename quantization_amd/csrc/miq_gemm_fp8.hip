@@ -98,38 +98,48 @@ __device__ __forceinline__ void store4(void* out, int64_t i, int n, bool vec, v4
     }
 }
 
-// Fills one LDS tile: K-tile kt of the ROWS rows at `rows`, `nrows` of which exist.  VEC: 16-byte LDS-DMA through a
-// descriptor that ends with the last row (K a multiple of 16); otherwise through registers, for any K and any alignment.
-template <int ROWS, int NWAVES, bool VEC>
+// Fills one LDS tile with 16-byte LDS-DMA: K-tile kt of the ROWS rows at `rows`, `nrows` of which exist (the others, and
+// columns past K, read as zeros).
+template <int ROWS, int NWAVES>
 __device__ __forceinline__ void stage_rows(const uint8_t* rows, int nrows, int K, int kt, char* tile, int wave, int lane) {
     constexpr int kPieces = ROWS / 8, kIters = (kPieces + NWAVES - 1) / NWAVES;
     const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(rows, static_cast<uint32_t>(nrows) * static_cast<uint32_t>(K));
-    const int slot = lane & 7;
 #pragma unroll
     for (int i = 0; i < kIters; ++i) {
         const int piece = wave + i * NWAVES;   // wave-uniform
         if (kPieces % NWAVES != 0 && piece >= kPieces) break;
         const int r = piece * 8 + (lane >> 3);
-        const int k = kt * kTileK + (slot ^ ((r >> 1) & 7)) * kChunk;
-        if constexpr (VEC) {
-            dma16(rsrc, tile + piece * (8 * kTileK), r < nrows && k < K ? static_cast<uint32_t>(r) * static_cast<uint32_t>(K) + k : kOob);
-        } else {
-            v4i v = {0, 0, 0, 0};
-            if (r < nrows && k < K) {
-                const uint8_t* p = rows + static_cast<int64_t>(r) * K + k;
-                if (K - k >= kChunk) {
-                    __builtin_memcpy(&v, p, kChunk);
-                } else {
-                    for (int b = 0; b < K - k; ++b) v[b >> 2] |= static_cast<int>(p[b]) << (8 * (b & 3));
-                }
-            }
-            *reinterpret_cast<v4i*>(tile + piece * (8 * kTileK) + lane * kChunk) = v;
-        }
+        const int k = kt * kTileK + ((lane & 7) ^ ((r >> 1) & 7)) * kChunk;
+        dma16(rsrc, tile + piece * (8 * kTileK), r < nrows && k < K ? static_cast<uint32_t>(r) * static_cast<uint32_t>(K) + k : kOob);
     }
 }
 
+// Rows of K bytes -> rows of `pitch` bytes (K rounded up to 16), zeros past K: one thread a 16-byte piece.
+__global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* __restrict__ src, int64_t rows, int K, int pitch,
+                                                       uint8_t* __restrict__ dst) {
+    const int per_row = pitch / kChunk;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * per_row; i += gridDim.x * 256ll) {
+        const int64_t r = i / per_row;
+        const int k = static_cast<int>(i % per_row) * kChunk;
+        const uint8_t* p = src + r * K + k;
+        v4i v = {0, 0, 0, 0};
+        if (K - k >= kChunk) {
+            __builtin_memcpy(&v, p, kChunk);
+        } else {
+            for (int b = 0; b < K - k; ++b) v[b >> 2] |= static_cast<int>(static_cast<uint32_t>(p[b]) << (8 * (b & 3)));
+        }
+        *reinterpret_cast<v4i*>(dst + i * kChunk) = v;
+    }
+}
+
+// The gate's activation, with the exponential and the error function in full fp32.
+__device__ __forceinline__ float gate_value(float g, int act) {
+    if (act == MIQ_ACT_SILU) return __fdiv_rn(g, 1.0f + expf(-g));
+    return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+}
+
 // BM x BN outputs a workgroup, two K-tile buffers, one barrier a K-tile.
-template <int BM, int BN, int WAVES_M, int WAVES_N, int OUT, bool VEC>
+template <int BM, int BN, int WAVES_M, int WAVES_N, int OUT>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(Fp8Args g) {
     constexpr int NWAVES = WAVES_M * WAVES_N;
     constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, FM = WM / 16, FN = WN / 16;
@@ -167,8 +177,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
     }
     auto stage = [&](int kt) {
         char* buf = smem + (kt & 1) * STAGE;
-        stage_rows<BM, NWAVES, VEC>(xrows, mrows, g.K, kt, buf, wave, lane);
-        stage_rows<BN, NWAVES, VEC>(wrows, nrows, g.K, kt, buf + BM * kTileK, wave, lane);
+        stage_rows<BM, NWAVES>(xrows, mrows, g.K, kt, buf, wave, lane);
+        stage_rows<BN, NWAVES>(wrows, nrows, g.K, kt, buf + BM * kTileK, wave, lane);
     };
     if (kt0 < kt1) stage(kt0);
     __syncthreads();
@@ -209,13 +219,237 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
     }
 }
 
-// ---- the gated product's second half -------------------------------------------------------------------------------
-// h = act(sum of the gate's slabs) * (sum of the up projection's), in blocks: sixteen lanes a block of one row.
-__device__ __forceinline__ float gate_value(float g, int act) {
-    if (act == MIQ_ACT_SILU) return __fdiv_rn(g, 1.0f + expf(-g));
-    return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+// ---- 256 x 256 outputs a workgroup: large products -----------------------------------------------------------------
+// Eight waves, 2 (rows) x 4 (columns), a wave owns 128 x 64 outputs: eight row fragments by four column fragments.  A K-tile
+// is 64 KiB of LDS (256 rows of x, 256 of w), double-buffered; one barrier a K-tile: past it tile t has landed for everyone
+// and the buffer of tile t - 1 is free, so the DMA of tile t + 1 has the whole of tile t's matrix work to land in.
+//
+// Within a K-tile a wave keeps the four column fragments and walks its row fragments; the sums of row fragment i - 1 are
+// scaled into the accumulators between the first matrix instructions of row fragment i, so that the vector work (the
+// scaling, and the widening of codes) runs in the shadow of the matrix pipe without a second set of sums.
+//
+// GATED: the tile is 128 columns of both weights, a wave's column fragments 0, 1 the gate's and 2, 3 the up projection's
+// same 32 columns, so that a lane holds both factors of its outputs and the 128 columns are one block of the result.
+template <bool NATIVE>
+struct BigTypes;
+template <>
+struct BigTypes<true> {
+    using Frag = Codes;
+};
+template <>
+struct BigTypes<false> {
+    using Frag = Widened;
+};
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ v4f first_mfma(const Codes& w, const Codes& x) {
+    const v8i a = __builtin_shufflevector(w.c[0], w.c[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    const v8i b = __builtin_shufflevector(x.c[0], x.c[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ v4f first_mfma(const Widened& w, const Widened& x) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.h[0], x.h[0], v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+}
+template <bool NATIVE>
+__device__ __forceinline__ auto operand(const Codes& c) {
+    if constexpr (NATIVE) return c;
+    else return widen(c);
 }
 
+struct GatedOut {
+    uint8_t* q;      // [M, N]
+    float* scale;    // [ceil(N / 128), M]
+    int act;
+};
+
+template <int OUT, bool GATED, bool NATIVE>
+__global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut go) {
+    constexpr int kHalf = 256 * kTileK, kStage = 2 * kHalf, kCols = GATED ? 128 : 256;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 2, wn = wave & 3;
+    int tm, tn;
+    tile_coords(blockIdx.x, gridDim.x, g.tiles_m, g.tiles_n, 8, tm, tn);
+    const int64_t m0 = static_cast<int64_t>(tm) * 256;
+    const int n0 = tn * kCols;
+    const int mrows = static_cast<int>(g.M - m0 < 256 ? g.M - m0 : 256), nrows = g.N - n0 < kCols ? g.N - n0 : kCols;
+
+    // Staging: a wave-instruction moves 8 rows x 128 B; wave v moves rows v * 8 + 64 i, i = 0 .. 3, of each operand.
+    const int srow = wave * 8 + (lane >> 3);
+    const int cbyte = ((lane & 7) ^ ((srow >> 1) & 7)) * kChunk;
+    const uint32_t off0 = static_cast<uint32_t>(srow) * static_cast<uint32_t>(g.K) + cbyte;
+    const uint32_t step = 64u * static_cast<uint32_t>(g.K);
+    const __amdgpu_buffer_rsrc_t rx = make_rsrc(g.x + m0 * g.K, static_cast<uint32_t>(mrows) * static_cast<uint32_t>(g.K));
+    const __amdgpu_buffer_rsrc_t rw0 = make_rsrc(g.w[0] + static_cast<int64_t>(n0) * g.K, static_cast<uint32_t>(nrows) * static_cast<uint32_t>(g.K));
+    const __amdgpu_buffer_rsrc_t rw1 = make_rsrc(g.w[GATED ? 1 : 0] + static_cast<int64_t>(n0) * g.K, static_cast<uint32_t>(nrows) * static_cast<uint32_t>(g.K));
+    auto stage = [&](int kt) {
+        char* buf = smem + (kt & 1) * kStage;
+        const int k = kt * kTileK;
+        const bool in = k + cbyte < g.K;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            // rows past the matrix lie past the descriptor's end and read as zeros
+            dma16(rx, buf + (wave + 8 * i) * (8 * kTileK), in ? off0 + i * step + k : kOob);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            char* dst = buf + kHalf + (wave + 8 * i) * (8 * kTileK);
+            if constexpr (GATED) dma16(i < 2 ? rw0 : rw1, dst, in ? off0 + (i & 1) * step + k : kOob);
+            else dma16(rw0, dst, in ? off0 + i * step + k : kOob);
+        }
+    };
+
+    // The scales of this lane's rows (one of each fragment) for K-tile kt, times nothing yet; rows past the end read as 0.
+    const uint32_t soff = static_cast<uint32_t>(wm * 128 + (lane & 15)) * 4;
+    auto row_scales = [&](int kt, float (&s)[8]) {
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(g.xs + static_cast<int64_t>(kt) * g.M + m0, static_cast<uint32_t>(mrows) * 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, soff + i * 64, 0, 0));
+    };
+    const int nblock = GATED ? tn : tn * 2 + (wn >> 1);
+    const int nblocks = (g.N + 127) / 128, nb = nblock < nblocks ? nblock : nblocks - 1;   // (columns past N: any scale)
+    const float* ws0 = g.ws[0] + static_cast<int64_t>(nb) * g.kblocks;
+    const float* ws1 = g.ws[GATED ? 1 : 0] + static_cast<int64_t>(nb) * g.kblocks;
+
+    // Column fragment j of this wave inside the staged 256 rows of w.
+    const int lo0 = frag_lane_offset(lane, 0), lo1 = frag_lane_offset(lane, 1);
+    auto w_row = [&](int j) { return GATED ? (j >> 1) * 128 + wn * 32 + (j & 1) * 16 : wn * 64 + j * 16; };
+    auto read = [&](const char* tile, int row) { return Codes{{lds_read16(tile + row * kTileK + lo0), lds_read16(tile + row * kTileK + lo1)}}; };
+
+    using Frag = typename BigTypes<NATIVE>::Frag;
+    v4f acc[8][4] = {};
+    v4f c[4] = {};
+    float s_cur[8], s_last0 = 0.f, s_last1 = 0.f;   // s_last: the scales of the sums still in c (row fragment 7 of the tile before)
+    const int nt = g.kblocks;
+    if (nt > 0) stage(0);
+    for (int t = 0; t < nt; ++t) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's share of tile t
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        row_scales(t, s_cur);   // (ahead of the DMA: their wait leaves it in flight)
+        if (t + 1 < nt) stage(t + 1);
+        const float sw0 = ws0[t], sw1 = GATED ? ws1[t] : sw0;
+        const char* xt = smem + (t & 1) * kStage + wm * 128 * kTileK;
+        const char* wt = smem + (t & 1) * kStage + kHalf;
+        Codes raw = read(xt, 0);
+        Frag wf[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) wf[j] = operand<NATIVE>(read(wt, w_row(j)));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const Frag xf = operand<NATIVE>(raw);
+            if (i < 7) raw = read(xt, (i + 1) * 16);
+            const int p = i ? i - 1 : 7;   // the row fragment whose sums are in c
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                add_scaled(acc[p][j], c[j], GATED && j >= 2 ? s_last1 : s_last0);
+                c[j] = first_mfma(wf[j], xf);
+            }
+            if constexpr (!NATIVE) {
+#pragma unroll
+                for (int h = 1; h < 4; ++h)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) c[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j].h[h], xf.h[h], c[j], 0, 0, 0);
+            }
+            s_last0 = s_cur[i] * sw0;
+            if constexpr (GATED) s_last1 = s_cur[i] * sw1;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) add_scaled(acc[7][j], c[j], GATED && j >= 2 ? s_last1 : s_last0);
+
+    // Results of a fragment: 4 * (lane >> 4) + register -> column, lane & 15 -> row.
+    const int64_t mw = m0 + wm * 128 + (lane & 15);
+    if constexpr (GATED) {
+        // The tile's 128 columns are a block of the result.  Its maximum for each row: over the lane's eight values, the
+        // four lanes of the row, and the four waves of the row through LDS.
+        __syncthreads();   // every wave has read its last K-tile
+        uint32_t* tops = reinterpret_cast<uint32_t*>(smem);   // [4][256]
+        auto top_of = [&](int i, auto bits) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t b = bits(acc[i][j][e]);
+                    top = b > top ? b : top;
+                }
+            uint32_t o = __shfl_xor(top, 16, 64);
+            top = o > top ? o : top;
+            o = __shfl_xor(top, 32, 64);
+            top = o > top ? o : top;
+            if (lane < 16) tops[wn * 256 + wm * 128 + i * 16 + lane] = top;
+        };
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = gate_value(acc[i][j][e], go.act) * acc[i][j + 2][e];
+            top_of(i, magnitude_bits);
+        }
+        __syncthreads();
+        auto row_top = [&](int i) {
+            const uint32_t* t = tops + wm * 128 + i * 16 + (lane & 15);
+            uint32_t top = t[0];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) top = t[w * 256] > top ? t[w * 256] : top;
+            return top;
+        };
+        bool spoiled = false;   // some value of this wave's rows is not finite: the same in the four waves of these rows
+#pragma unroll
+        for (int i = 0; i < 8; ++i) spoiled |= row_top(i) >= kInfBits;
+        spoiled = __any(spoiled);
+        __syncthreads();
+        if (spoiled) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top_of(i, finite_magnitude_bits);
+        }
+        __syncthreads();
+        const bool vec = (g.N & 3) == 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int64_t m = mw + i * 16;
+            const BlockScale s = block_scale(row_top(i));
+            if (m >= g.M) continue;
+            if (wn == 0 && lane < 16) go.scale[static_cast<int64_t>(tn) * g.M + m] = s.scale;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int n = n0 + wn * 32 + j * 16 + (lane >> 4) * 4;
+                float f[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[e] = __fmul_rn(spoiled ? infinite_to_nan(acc[i][j][e]) : acc[i][j][e], s.inv);
+                const uint32_t code = pack4_e4m3(f[0], f[1], f[2], f[3]);
+                uint8_t* o = go.q + m * g.N + n;
+                if (vec && n + 3 < g.N) *reinterpret_cast<uint32_t*>(o) = code;
+                else
+                    for (int e = 0; e < 4; ++e)
+                        if (n + e < g.N) o[e] = static_cast<uint8_t>(code >> (8 * e));
+            }
+        }
+    } else {
+        const bool vec = (g.N & 3) == 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int n = n0 + wn * 64 + j * 16 + (lane >> 4) * 4;
+            if (n >= g.N) continue;
+            v4f b = {0.f, 0.f, 0.f, 0.f};
+            if (g.bias)
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < g.N) b[e] = g.bias[n + e];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int64_t m = mw + i * 16;
+                if (m < g.M) store4<OUT>(g.out, m * g.N + n, g.N - n, vec, acc[i][j] + b);
+            }
+        }
+    }
+}
+
+// ---- the gated product's second half -------------------------------------------------------------------------------
+// h = act(sum of the gate's slabs) * (sum of the up projection's), in blocks: sixteen lanes a block of one row.
 __global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict__ slabs, int splits, int64_t M, int N, int nblocks,
                                                          int act, uint8_t* __restrict__ q, float* __restrict__ scale) {
     const int lane = threadIdx.x & 15;
@@ -253,35 +487,100 @@ int check_sizes(const char* who, int64_t M, int64_t N, int64_t K) {
     return MIQ_OK;
 }
 
-Fp8Args make_args(const uint8_t* x, const float* xs, const uint8_t* w, const float* ws, int64_t M, int64_t N, int64_t K) {
+size_t align256(int64_t n) { return static_cast<size_t>(round_up(n, 256)); }
+
+// A row length that is no multiple of 16 bytes cannot be staged in 16-byte pieces: both operands are first copied to rows of
+// a multiple of 16, zero-filled (codes of 0 add nothing), at the front of the workspace.
+int64_t pitch_of(int64_t K) { return round_up(K, kChunk); }
+size_t padded_bytes(int64_t M, int64_t N, int64_t weights, int64_t K) {
+    return K % kChunk == 0 ? 0 : align256(M * pitch_of(K)) + static_cast<size_t>(weights) * align256(N * pitch_of(K));
+}
+const uint8_t* pad_rows(const uint8_t* src, int64_t rows, int64_t K, char*& at, hipStream_t st) {
+    uint8_t* dst = reinterpret_cast<uint8_t*>(at);
+    const int64_t pieces = rows * (pitch_of(K) / kChunk), groups = ceil_div(pieces, 256);
+    pad_rows_kernel<<<static_cast<unsigned>(groups < 16384 ? groups : 16384), 256, 0, st>>>(src, rows, static_cast<int>(K),
+                                                                                            static_cast<int>(pitch_of(K)), dst);
+    at += align256(rows * pitch_of(K));
+    return dst;
+}
+
+// What a product is cut into: which kernel, and how much workspace it needs behind the padded operands.
+struct Fp8Plan {
+    bool big;        // 256 x 256 tiles
+    size_t slabs;    // bytes
+};
+
+// Large products: at least this many 256 x 256 tiles run on the 256 x 256 kernel.
+constexpr int64_t kBigTiles = 128;
+
+Fp8Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
+    Fp8Plan p{};
+    p.big = M > 128 && ceil_div(M, 256) * ceil_div(N, gated ? 128 : 256) >= kBigTiles;
+    if (gated && !p.big) p.slabs = static_cast<size_t>(2 * 4 * M * N);
+    return p;
+}
+
+template <int OUT>
+int launch_tiles(Fp8Args g, int products, hipStream_t st) {
+    constexpr int BM = 64, BN = 64, kLds = 2 * (BM + BN) * kTileK;
+    g.tiles_m = static_cast<int>(ceil_div(g.M, BM));
+    g.tiles_n = static_cast<int>(ceil_div(g.N, BN));
+    const dim3 grid(static_cast<unsigned>(g.tiles_m) * g.tiles_n, 1, products);
+    gemm_fp8_tile_kernel<BM, BN, 2, 2, OUT><<<grid, 256, kLds, st>>>(g);
+    return check_launch("gemm_fp8_tile_kernel");
+}
+
+template <int OUT, bool GATED, bool NATIVE>
+int launch_big(Fp8Args g, GatedOut go, hipStream_t st) {
+    constexpr int kLds = 2 * 2 * 256 * kTileK;
+    g.tiles_m = static_cast<int>(ceil_div(g.M, 256));
+    g.tiles_n = static_cast<int>(ceil_div(g.N, GATED ? 128 : 256));
+    const void* fn = reinterpret_cast<const void*>(&gemm_fp8_256_kernel<OUT, GATED, NATIVE>);
+    if (int rc = allow_lds(fn, kLds)) return rc;
+    gemm_fp8_256_kernel<OUT, GATED, NATIVE><<<static_cast<unsigned>(g.tiles_m) * g.tiles_n, 512, kLds, st>>>(g, go);
+    return check_launch("gemm_fp8_256_kernel");
+}
+
+// Checks that both products share; `weights` of them, 1 or 2.
+size_t workspace_of(const char* who, int64_t M, int64_t N, int64_t K, bool gated) {
+    if (check_sizes(who, M, N, K) != MIQ_OK || M == 0 || N == 0) return 0;
+    return padded_bytes(M, N, gated ? 2 : 1, K) + make_plan(M, N, K, gated).slabs;
+}
+int check_workspace(const char* who, size_t need, const void* workspace, size_t bytes) {
+    MIQ_REQUIRE(need == 0 || (workspace && bytes >= need), MIQ_EWORKSPACE, "%s: %zu bytes of workspace needed, %zu given", who, need,
+                workspace ? bytes : 0);
+    MIQ_REQUIRE(aligned(workspace, 256), MIQ_EALIGN, "%s: workspace must be 256-byte aligned", who);
+    return MIQ_OK;
+}
+
+// The arguments of a launch, operands padded where they need it; `at` is moved past what that took of the workspace.
+Fp8Args make_args(const uint8_t* x, const float* xs, const uint8_t* w, const float* ws, const uint8_t* w2, const float* ws2, int64_t M,
+                  int64_t N, int64_t K, char*& at, hipStream_t st) {
     Fp8Args g{};
-    g.x = x;
+    const bool pad = K % kChunk != 0;
+    g.x = pad ? pad_rows(x, M, K, at, st) : x;
     g.xs = xs;
-    g.w[0] = w;
+    g.w[0] = pad ? pad_rows(w, N, K, at, st) : w;
+    g.w[1] = pad && w2 ? pad_rows(w2, N, K, at, st) : w2;
     g.ws[0] = ws;
+    g.ws[1] = ws2;
     g.M = M;
     g.N = static_cast<int>(N);
-    g.K = static_cast<int>(K);
+    g.K = static_cast<int>(pitch_of(K));
     g.kblocks = static_cast<int>(ceil_div(K, kTileK));
     return g;
 }
 
 template <int OUT>
-int launch_tiles(Fp8Args g, int products, bool vec, hipStream_t st) {
-    constexpr int BM = 64, BN = 64, kLds = 2 * (BM + BN) * kTileK;
-    g.tiles_m = static_cast<int>(ceil_div(g.M, BM));
-    g.tiles_n = static_cast<int>(ceil_div(g.N, BN));
-    const dim3 grid(static_cast<unsigned>(g.tiles_m) * g.tiles_n, 1, products);
-    if (vec) gemm_fp8_tile_kernel<BM, BN, 2, 2, OUT, true><<<grid, 256, kLds, st>>>(g);
-    else gemm_fp8_tile_kernel<BM, BN, 2, 2, OUT, false><<<grid, 256, kLds, st>>>(g);
-    return check_launch("gemm_fp8_tile_kernel");
+int run_product(const Fp8Args& g, const Fp8Plan& plan, hipStream_t st) {
+    if (plan.big) return launch_big<OUT, false, OUT != MIQ_F32>(g, {}, st);
+    return launch_tiles<OUT>(g, 1, st);
 }
 
 }  // namespace
 
 extern "C" size_t miq_gemm_fp8_workspace(int64_t M, int64_t N, int64_t K) {
-    if (check_sizes("miq_gemm_fp8_workspace", M, N, K) != MIQ_OK) return 0;
-    return 0;
+    return workspace_of("miq_gemm_fp8_workspace", M, N, K, false);
 }
 
 extern "C" int miq_gemm_fp8(const uint8_t* x, const float* x_scale, const uint8_t* w, const float* w_scale, int64_t M, int64_t N,
@@ -294,18 +593,21 @@ extern "C" int miq_gemm_fp8(const uint8_t* x, const float* x_scale, const uint8_
     MIQ_REQUIRE(out && (K == 0 || (x && x_scale && w && w_scale)), MIQ_EINVAL, "miq_gemm_fp8: null pointer");
     MIQ_REQUIRE(aligned(x_scale, 4) && aligned(w_scale, 4) && aligned(bias, 4) && aligned(out, 16), MIQ_EALIGN,
                 "miq_gemm_fp8: scales and bias must be 4-byte, out 16-byte aligned");
-    Fp8Args g = make_args(x, x_scale, w, w_scale, M, N, K);
+    MIQ_REQUIRE(K % kChunk != 0 || (aligned(x, 16) && aligned(w, 16)), MIQ_EALIGN, "miq_gemm_fp8: x and w must be 16-byte aligned");
+    if (int rc = check_workspace("miq_gemm_fp8", miq_gemm_fp8_workspace(M, N, K), workspace, workspace_bytes)) return rc;
+    const hipStream_t st = as_stream(stream);
+    char* at = static_cast<char*>(workspace);
+    Fp8Args g = make_args(x, x_scale, w, w_scale, nullptr, nullptr, M, N, K, at, st);
     g.bias = bias;
     g.out = out;
-    const bool vec = K % 16 == 0 && aligned(x, 16) && aligned(w, 16);
-    if (out_dtype == MIQ_F32) return launch_tiles<MIQ_F32>(g, 1, vec, as_stream(stream));
-    if (out_dtype == MIQ_F16) return launch_tiles<MIQ_F16>(g, 1, vec, as_stream(stream));
-    return launch_tiles<MIQ_BF16>(g, 1, vec, as_stream(stream));
+    const Fp8Plan plan = make_plan(M, N, K, false);
+    if (out_dtype == MIQ_F32) return run_product<MIQ_F32>(g, plan, st);
+    if (out_dtype == MIQ_F16) return run_product<MIQ_F16>(g, plan, st);
+    return run_product<MIQ_BF16>(g, plan, st);
 }
 
 extern "C" size_t miq_gated_fp8_workspace(int64_t M, int64_t N, int64_t K) {
-    if (check_sizes("miq_gated_fp8_workspace", M, N, K) != MIQ_OK) return 0;
-    return static_cast<size_t>(2 * 4 * M * N);
+    return workspace_of("miq_gated_fp8_workspace", M, N, K, true);
 }
 
 extern "C" int miq_gated_fp8(const uint8_t* x, const float* x_scale, const uint8_t* w_gate, const float* gate_scale,
@@ -316,22 +618,22 @@ extern "C" int miq_gated_fp8(const uint8_t* x, const float* x_scale, const uint8
     if (M == 0 || N == 0) return MIQ_OK;
     MIQ_REQUIRE(q && scale && (K == 0 || (x && x_scale && w_gate && gate_scale && w_up && up_scale)), MIQ_EINVAL,
                 "miq_gated_fp8: null pointer");
-    MIQ_REQUIRE(aligned(x_scale, 4) && aligned(gate_scale, 4) && aligned(up_scale, 4) && aligned(scale, 4), MIQ_EALIGN,
-                "miq_gated_fp8: scales must be 4-byte aligned");
-    const size_t need = miq_gated_fp8_workspace(M, N, K);
-    MIQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), MIQ_EWORKSPACE, "miq_gated_fp8: %zu bytes of workspace needed, %zu given",
-                need, workspace_bytes);
-    MIQ_REQUIRE(aligned(workspace, 256), MIQ_EALIGN, "miq_gated_fp8: workspace must be 256-byte aligned");
-    Fp8Args g = make_args(x, x_scale, w_gate, gate_scale, M, N, K);
-    g.w[1] = w_up;
-    g.ws[1] = up_scale;
-    g.out = workspace;
-    g.kt_per_split = g.kblocks > 0 ? g.kblocks : 1;
-    const bool vec = K % 16 == 0 && aligned(x, 16) && aligned(w_gate, 16) && aligned(w_up, 16);
-    if (int rc = launch_tiles<MIQ_F32>(g, 2, vec, as_stream(stream))) return rc;
+    MIQ_REQUIRE(aligned(x_scale, 4) && aligned(gate_scale, 4) && aligned(up_scale, 4) && aligned(scale, 4) && aligned(q, 16), MIQ_EALIGN,
+                "miq_gated_fp8: scales must be 4-byte, q 16-byte aligned");
+    MIQ_REQUIRE(K % kChunk != 0 || (aligned(x, 16) && aligned(w_gate, 16) && aligned(w_up, 16)), MIQ_EALIGN,
+                "miq_gated_fp8: x and the weights must be 16-byte aligned");
+    if (int rc = check_workspace("miq_gated_fp8", miq_gated_fp8_workspace(M, N, K), workspace, workspace_bytes)) return rc;
+    const hipStream_t st = as_stream(stream);
+    char* at = static_cast<char*>(workspace);
+    Fp8Args g = make_args(x, x_scale, w_gate, gate_scale, w_up, up_scale, M, N, K, at, st);
+    const Fp8Plan plan = make_plan(M, N, K, true);
+    if (plan.big) return launch_big<MIQ_F32, true, false>(g, {q, scale, act}, st);
     const int nblocks = static_cast<int>(ceil_div(N, 128));
     MIQ_REQUIRE(ceil_div(M * nblocks, 16) < (1ll << 24), MIQ_ERANGE, "miq_gated_fp8: too many blocks");
-    gated_join_kernel<<<static_cast<unsigned>(ceil_div(M * nblocks, 16)), 256, 0, as_stream(stream)>>>(
-        static_cast<const float*>(workspace), 1, M, g.N, nblocks, act, q, scale);
+    g.out = at;
+    g.kt_per_split = g.kblocks > 0 ? g.kblocks : 1;
+    if (int rc = launch_tiles<MIQ_F32>(g, 2, st)) return rc;
+    gated_join_kernel<<<static_cast<unsigned>(ceil_div(M * nblocks, 16)), 256, 0, st>>>(reinterpret_cast<const float*>(at), 1, M, g.N,
+                                                                                     nblocks, act, q, scale);
     return check_launch("gated_join_kernel");
 }

@@ -181,6 +181,48 @@ def test_linear(out, m, n, k):
     assert bool((off <= tol)[fits].all()), float((off / tol)[fits].max())
 
 
+LARGE = [(2048, 4100, 272), (300, 16260, 130), (1025, 6500, 1040)]
+
+
+@pytest.mark.parametrize("out", FLOATS)
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_large_linear(out, m, n, k):
+    """Sizes of at least 128 tiles of 256 x 256.  fp32 outputs keep fp32 sums; 16-bit outputs come from the 8-bit matrix
+    instruction, which drops of each of eight neighbouring products less than 2^-13 of the largest: 2^-10 of the sum of
+    magnitudes at most."""
+    from quantization_amd import block_fp8 as F
+    xq, xs = codes(m, k, 1)
+    wq, ws = codes(n, k, 2, weight=True)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(n))
+    y = F.linear_fp8(xq.cuda(), xs.cuda(), wq.cuda(), ws.cuda(), bias.cuda(), out)
+    ref, mag = R.product(xq, xs, wq, ws)
+    ref = ref + bias.double()
+    err = R.product_error(mag, k) + (0 if out == torch.float32 else 2.0 ** -10 * mag) + 2.0 ** -24 * ref.abs()
+    off = (y.cpu().double() - ref).abs()
+    tol = err + torch.finfo(out).eps / 2 * (ref.abs() + err) + torch.finfo(out).smallest_normal * torch.finfo(out).eps
+    fits = ref.abs() < torch.finfo(out).max * 0.99
+    assert bool((off <= tol)[fits].all()), float((off / tol)[fits].max())
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("m,n,k", [(300, 8132, 272), (1030, 3300, 130)])
+def test_large_gated(act, m, n, k):
+    from quantization_amd import block_fp8 as F
+    xq, xs = codes(m, k, 3)
+    gq, gs = codes(n, k, 4, weight=True)
+    uq, us = codes(n, k, 5, weight=True)
+    gs = gs * 0.05
+    x = xq.float()
+    x[7] = math.nan      # a spoiled row, and a row of zeros
+    x[290] = 0
+    xq = x.to(torch.float8_e4m3fn)
+    q, s = F.gated_linear_fp8(xq.cuda(), xs.cuda(), gq.cuda(), gs.cuda(), uq.cuda(), us.cuda(), act)
+    assert bool(torch.isnan(q[7].float()).all()) and bool(torch.isfinite(s).all()) and not bool(q[290].float().any())
+    keep = [i for i in range(m) if i != 7]
+    y, dy = gated_reference(xq[keep], xs[:, keep], gq, gs, uq, us, act)
+    R.check_codes_of(q[keep], s[:, keep], y, dy)
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
 def test_gated(act, m, n, k):
