@@ -133,8 +133,9 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* __restrict
 }
 
 // The gate's activation, with the exponential and the error function in full fp32.
-__device__ __forceinline__ float gate_value(float g, int act) {
-    if (act == MIQ_ACT_SILU) return __fdiv_rn(g, 1.0f + expf(-g));
+template <int ACT>
+__device__ __forceinline__ float gate_value(float g) {
+    if constexpr (ACT == MIQ_ACT_SILU) return __fdiv_rn(g, 1.0f + expf(-g));
     return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
 }
 
@@ -220,13 +221,21 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
 }
 
 // ---- 256 x 256 outputs a workgroup: large products -----------------------------------------------------------------
-// Eight waves, 2 (rows) x 4 (columns), a wave owns 128 x 64 outputs: eight row fragments by four column fragments.  A K-tile
-// is 64 KiB of LDS (256 rows of x, 256 of w), double-buffered; one barrier a K-tile: past it tile t has landed for everyone
-// and the buffer of tile t - 1 is free, so the DMA of tile t + 1 has the whole of tile t's matrix work to land in.
+// Eight waves, 2 (rows) x 4 (columns), a wave owns 128 x 64 outputs: eight row fragments by four column fragments.
 //
 // Within a K-tile a wave keeps the four column fragments and walks its row fragments; the sums of row fragment i - 1 are
 // scaled into the accumulators between the first matrix instructions of row fragment i, so that the vector work (the
 // scaling, and the widening of codes) runs in the shadow of the matrix pipe without a second set of sums.
+//
+// A K-tile is two phases, A (read and widen the column fragments, row fragments 0-3) and B (4-7), a barrier before each.
+// Waves 4-7, the second wave of every SIMD, run one phase behind waves 0-3: while one wave reads and widens its column
+// fragments the other keeps the matrix pipe busy.  With barrier 2t at the start of A(t) for waves 0-3:
+//     after barrier 2t + 1 the rows x(t - 1) are read by nobody any more:  DMA of x(t + 2) into their slot (three slots)
+//     after barrier 2t     the rows w(t - 2 + 1) likewise:                 DMA of w(t + 1) (two slots)
+//     before barrier 2t    every wave has waited for its share of x(t) and w(t), issued three and two phases earlier; the
+//                          four pieces of x(t + 1) and two loads of scales may still be in flight
+// which fills the CU's 160 KiB of LDS with 32 KiB slots.  K-tiles past the end are requested out of range (zeros, no memory
+// traffic), so that every wave issues the same number of pieces.
 //
 // GATED: the tile is 128 columns of both weights, a wave's column fragments 0, 1 the gate's and 2, 3 the up projection's
 // same 32 columns, so that a lane holds both factors of its outputs and the 128 columns are one block of the result.
@@ -256,15 +265,16 @@ __device__ __forceinline__ auto operand(const Codes& c) {
     else return widen(c);
 }
 
+constexpr int kNoAct = -1;
 struct GatedOut {
     uint8_t* q;      // [M, N]
     float* scale;    // [ceil(N / 128), M]
-    int act;
 };
 
-template <int OUT, bool GATED, bool NATIVE>
+template <int OUT, int ACT, bool NATIVE>
 __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut go) {
-    constexpr int kHalf = 256 * kTileK, kStage = 2 * kHalf, kCols = GATED ? 128 : 256;
+    constexpr bool GATED = ACT != kNoAct;
+    constexpr int kSlot = 256 * kTileK, kCols = GATED ? 128 : 256;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -275,87 +285,141 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
     const int n0 = tn * kCols;
     const int mrows = static_cast<int>(g.M - m0 < 256 ? g.M - m0 : 256), nrows = g.N - n0 < kCols ? g.N - n0 : kCols;
 
-    // Staging: a wave-instruction moves 8 rows x 128 B; wave v moves rows v * 8 + 64 i, i = 0 .. 3, of each operand.
+    // Staging: a wave-instruction moves 8 rows x 128 B; wave v moves rows v * 8 + 64 i, i = 0 .. 3, of each operand.  K-tile
+    // and row group advance in the descriptor (scalar registers); a lane's offset stays.  Rows past the matrix lie past the
+    // descriptor's end and read as zeros.
     const int srow = wave * 8 + (lane >> 3);
     const int cbyte = ((lane & 7) ^ ((srow >> 1) & 7)) * kChunk;
     const uint32_t off0 = static_cast<uint32_t>(srow) * static_cast<uint32_t>(g.K) + cbyte;
-    const uint32_t step = 64u * static_cast<uint32_t>(g.K);
-    const __amdgpu_buffer_rsrc_t rx = make_rsrc(g.x + m0 * g.K, static_cast<uint32_t>(mrows) * static_cast<uint32_t>(g.K));
-    const __amdgpu_buffer_rsrc_t rw0 = make_rsrc(g.w[0] + static_cast<int64_t>(n0) * g.K, static_cast<uint32_t>(nrows) * static_cast<uint32_t>(g.K));
-    const __amdgpu_buffer_rsrc_t rw1 = make_rsrc(g.w[GATED ? 1 : 0] + static_cast<int64_t>(n0) * g.K, static_cast<uint32_t>(nrows) * static_cast<uint32_t>(g.K));
-    auto stage = [&](int kt) {
-        char* buf = smem + (kt & 1) * kStage;
+    // An operand's rows 0-127 and 128-255: first row, and how many exist (may be negative).
+    const uint8_t* const x0 = g.x + m0 * g.K;
+    const uint8_t* const w0 = g.w[0] + static_cast<int64_t>(n0) * g.K;
+    const uint8_t* const w128 = GATED ? g.w[1] + static_cast<int64_t>(n0) * g.K : w0 + 128ll * g.K;
+    const int w128_count = GATED ? nrows : nrows - 128;
+    // K-tile kt of the rows of w (else of x) to the 32 KiB at byte `slot` of LDS
+    auto stage = [&](bool of_w, int kt, int slot) {
         const int k = kt * kTileK;
-        const bool in = k + cbyte < g.K;
+        const uint32_t off = k + cbyte < g.K ? off0 : kOob;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            // rows past the matrix lie past the descriptor's end and read as zeros
-            dma16(rx, buf + (wave + 8 * i) * (8 * kTileK), in ? off0 + i * step + k : kOob);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            char* dst = buf + kHalf + (wave + 8 * i) * (8 * kTileK);
-            if constexpr (GATED) dma16(i < 2 ? rw0 : rw1, dst, in ? off0 + (i & 1) * step + k : kOob);
-            else dma16(rw0, dst, in ? off0 + i * step + k : kOob);
+            const uint8_t* rows = i < 2 ? (of_w ? w0 : x0) : (of_w ? w128 : x0 + 128ll * g.K);
+            const int count = i < 2 ? (of_w ? nrows : mrows) : (of_w ? w128_count : mrows - 128);
+            const int left = (count - (i & 1) * 64) * g.K - k;   // bytes from the piece's first row to the end
+            dma16(make_rsrc(rows + (i & 1) * 64ll * g.K + k, left > 0 ? left : 0), smem + slot + (wave + 8 * i) * (8 * kTileK), off);
         }
     };
+    auto x_slot = [](int slot) { return slot * kSlot; };
+    auto w_slot = [](int kt) { return (3 + (kt & 1)) * kSlot; };
 
-    // The scales of this lane's rows (one of each fragment) for K-tile kt, times nothing yet; rows past the end read as 0.
-    const uint32_t soff = static_cast<uint32_t>(wm * 128 + (lane & 15)) * 4;
-    auto row_scales = [&](int kt, float (&s)[8]) {
+    // The scales of the wave's 128 rows for one K-tile, a lane one of each half: lane l has row l of the half.  spread() gives
+    // every lane of a 16-lane row the scales of row fragment i, i.e. row 16 i + (lane & 15): three exchanges of 32- and
+    // 16-lane rows between two copies.  Rows past the end read as 0.
+    auto row_scales = [&](int kt, int half) {
         const __amdgpu_buffer_rsrc_t rs = make_rsrc(g.xs + static_cast<int64_t>(kt) * g.M + m0, static_cast<uint32_t>(mrows) * 4);
+        return __builtin_amdgcn_raw_buffer_load_b32(rs, static_cast<uint32_t>(wm * 128 + half * 64 + lane) * 4, 0, 0);
+    };
+    auto spread = [&](uint32_t v, float (&s)[4]) {
+        const auto halves = __builtin_amdgcn_permlane32_swap(v, v, false, false);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, soff + i * 64, 0, 0));
+        for (int h = 0; h < 2; ++h) {
+            const auto rows = __builtin_amdgcn_permlane16_swap(halves[h], halves[h], false, false);
+            s[2 * h] = __uint_as_float(rows[0]);
+            s[2 * h + 1] = __uint_as_float(rows[1]);
+        }
     };
     const int nblock = GATED ? tn : tn * 2 + (wn >> 1);
     const int nblocks = (g.N + 127) / 128, nb = nblock < nblocks ? nblock : nblocks - 1;   // (columns past N: any scale)
-    const float* ws0 = g.ws[0] + static_cast<int64_t>(nb) * g.kblocks;
-    const float* ws1 = g.ws[GATED ? 1 : 0] + static_cast<int64_t>(nb) * g.kblocks;
+    // (read through the scalar unit: a vector load here would be waited for behind the DMA issued before it)
+    using scalar_floats = const __attribute__((address_space(4))) float*;
+    const scalar_floats ws0 = (scalar_floats)(g.ws[0] + static_cast<int64_t>(nb) * g.kblocks);
+    const scalar_floats ws1 = (scalar_floats)(g.ws[GATED ? 1 : 0] + static_cast<int64_t>(nb) * g.kblocks);
 
     // Column fragment j of this wave inside the staged 256 rows of w.
     const int lo0 = frag_lane_offset(lane, 0), lo1 = frag_lane_offset(lane, 1);
     auto w_row = [&](int j) { return GATED ? (j >> 1) * 128 + wn * 32 + (j & 1) * 16 : wn * 64 + j * 16; };
-    auto read = [&](const char* tile, int row) { return Codes{{lds_read16(tile + row * kTileK + lo0), lds_read16(tile + row * kTileK + lo1)}}; };
+    auto read = [&](int tile, int row) {
+        return Codes{{lds_read16(smem + tile + lo0 + row * kTileK), lds_read16(smem + tile + lo1 + row * kTileK)}};
+    };
 
     using Frag = typename BigTypes<NATIVE>::Frag;
     v4f acc[8][4] = {};
     v4f c[4] = {};
-    float s_cur[8], s_last0 = 0.f, s_last1 = 0.f;   // s_last: the scales of the sums still in c (row fragment 7 of the tile before)
+    float s_cur[4], s_last0 = 0.f, s_last1 = 0.f;   // s_last: the scales of the sums still in c (row fragment 7 of the tile before)
     const int nt = g.kblocks;
-    if (nt > 0) stage(0);
-    for (int t = 0; t < nt; ++t) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's share of tile t
+    Frag wf[4];
+    Codes raw;
+    auto rows_step = [&](auto step, int xt, uint32_t sv, float sw0, float sw1) {
+        constexpr int i = decltype(step)::value;
+        const Frag xf = operand<NATIVE>(raw);
+        if (i < 7) raw = read(xt, (i + 1) * 16);
+        const int p = i ? i - 1 : 7;   // the row fragment whose sums are in c
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            add_scaled(acc[p][j], c[j], GATED && j >= 2 ? s_last1 : s_last0);
+            asm volatile("" : "+v"(acc[p][j]));   // here and not at the loop's end, with all sums kept until then
+            c[j] = first_mfma(wf[j], xf);
+        }
+        if constexpr (!NATIVE) {
+#pragma unroll
+            for (int h = 1; h < 4; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j].h[h], xf.h[h], c[j], 0, 0, 0);
+        }
+        if (i % 4 == 0) spread(sv, s_cur);
+        s_last0 = s_cur[i % 4] * sw0;
+        if constexpr (GATED) s_last1 = s_cur[i % 4] * sw1;
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto barrier = [&] {
+        asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        row_scales(t, s_cur);   // (ahead of the DMA: their wait leaves it in flight)
-        if (t + 1 < nt) stage(t + 1);
-        const float sw0 = ws0[t], sw1 = GATED ? ws1[t] : sw0;
-        const char* xt = smem + (t & 1) * kStage + wm * 128 * kTileK;
-        const char* wt = smem + (t & 1) * kStage + kHalf;
-        Codes raw = read(xt, 0);
-        Frag wf[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) wf[j] = operand<NATIVE>(read(wt, w_row(j)));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const Frag xf = operand<NATIVE>(raw);
-            if (i < 7) raw = read(xt, (i + 1) * 16);
-            const int p = i ? i - 1 : 7;   // the row fragment whose sums are in c
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                add_scaled(acc[p][j], c[j], GATED && j >= 2 ? s_last1 : s_last0);
-                c[j] = first_mfma(wf[j], xf);
-            }
-            if constexpr (!NATIVE) {
-#pragma unroll
-                for (int h = 1; h < 4; ++h)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) c[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j].h[h], xf.h[h], c[j], 0, 0, 0);
-            }
-            s_last0 = s_cur[i] * sw0;
-            if constexpr (GATED) s_last1 = s_cur[i] * sw1;
-            __builtin_amdgcn_sched_barrier(0);
+    };
+    using std::integral_constant;
+    if (nt > 0) {
+        stage(false, 0, x_slot(0));
+        stage(true, 0, w_slot(0));
+        stage(false, 1, x_slot(1));
+        uint32_t sv0 = row_scales(0, 0), sv1 = row_scales(0, 1);
+        asm volatile("s_waitcnt vmcnt(6)" ::: "memory");   // x(0), w(0)
+        barrier();
+        int group = wm;
+        if (group == 1) {
+            stage(true, 1, w_slot(1));
+            barrier();
         }
+        int slot = 0;   // of x(t)
+        for (int t = 0; t < nt; ++t) {
+            asm volatile("" : "+s"(group));   // (one loop for both groups: the body is not worth duplicating)
+            const int xt = x_slot(slot) + wm * 128 * kTileK, wt = w_slot(t);
+            const int ahead = slot == 0 ? 2 : slot - 1;   // of x(t + 2), and of x(t - 1)
+            slot = slot == 2 ? 0 : slot + 1;
+            const float sw0 = ws0[t], sw1 = GATED ? ws1[t] : sw0;
+            // phase A
+            stage(group == 0, group ? t + 2 : t + 1, group ? x_slot(ahead) : w_slot(t + 1));
+            raw = read(xt, 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) wf[j] = operand<NATIVE>(read(wt, w_row(j)));
+            rows_step(integral_constant<int, 0>{}, xt, sv0, sw0, sw1);
+            rows_step(integral_constant<int, 1>{}, xt, sv0, sw0, sw1);
+            rows_step(integral_constant<int, 2>{}, xt, sv0, sw0, sw1);
+            rows_step(integral_constant<int, 3>{}, xt, sv0, sw0, sw1);
+            if (group) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");   // x(t + 1), w(t + 1); x(t + 2) stays in flight
+            barrier();
+            // phase B
+            stage(group != 0, t + 2, group ? w_slot(t + 2) : x_slot(ahead));
+            const int tn1 = t + 1 < nt ? t + 1 : t;
+            sv0 = row_scales(tn1, 0);
+            rows_step(integral_constant<int, 4>{}, xt, sv1, sw0, sw1);
+            sv1 = row_scales(tn1, 1);
+            rows_step(integral_constant<int, 5>{}, xt, sv1, sw0, sw1);
+            rows_step(integral_constant<int, 6>{}, xt, sv1, sw0, sw1);
+            rows_step(integral_constant<int, 7>{}, xt, sv1, sw0, sw1);
+            if (!group) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+            barrier();
+        }
+        if (wm == 0) barrier();   // every wave executes the same number of barriers
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the pieces requested for K-tiles past the end
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) add_scaled(acc[7][j], c[j], GATED && j >= 2 ? s_last1 : s_last0);
@@ -387,7 +451,7 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = gate_value(acc[i][j][e], go.act) * acc[i][j + 2][e];
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = gate_value<ACT>(acc[i][j][e]) * acc[i][j + 2][e];
             top_of(i, magnitude_bits);
         }
         __syncthreads();
@@ -450,8 +514,9 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
 
 // ---- the gated product's second half -------------------------------------------------------------------------------
 // h = act(sum of the gate's slabs) * (sum of the up projection's), in blocks: sixteen lanes a block of one row.
+template <int ACT>
 __global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict__ slabs, int splits, int64_t M, int N, int nblocks,
-                                                         int act, uint8_t* __restrict__ q, float* __restrict__ scale) {
+                                                         uint8_t* __restrict__ q, float* __restrict__ scale) {
     const int lane = threadIdx.x & 15;
     const int64_t id = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
     const int64_t m = id / nblocks;
@@ -467,7 +532,7 @@ __global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict
             float gate = 0.0f, up = 0.0f;
             for (int s = 0; s < splits; ++s) gate += slabs[s * size + o];
             for (int s = 0; s < splits; ++s) up += slabs[(splits + s) * size + o];
-            h[i] = gate_value(gate, act) * up;
+            h[i] = gate_value<ACT>(gate) * up;
         }
     }
     uint32_t c[2];
@@ -530,14 +595,14 @@ int launch_tiles(Fp8Args g, int products, hipStream_t st) {
     return check_launch("gemm_fp8_tile_kernel");
 }
 
-template <int OUT, bool GATED, bool NATIVE>
+template <int OUT, int ACT, bool NATIVE>
 int launch_big(Fp8Args g, GatedOut go, hipStream_t st) {
-    constexpr int kLds = 2 * 2 * 256 * kTileK;
+    constexpr int kLds = 5 * 256 * kTileK;
     g.tiles_m = static_cast<int>(ceil_div(g.M, 256));
-    g.tiles_n = static_cast<int>(ceil_div(g.N, GATED ? 128 : 256));
-    const void* fn = reinterpret_cast<const void*>(&gemm_fp8_256_kernel<OUT, GATED, NATIVE>);
+    g.tiles_n = static_cast<int>(ceil_div(g.N, ACT != kNoAct ? 128 : 256));
+    const void* fn = reinterpret_cast<const void*>(&gemm_fp8_256_kernel<OUT, ACT, NATIVE>);
     if (int rc = allow_lds(fn, kLds)) return rc;
-    gemm_fp8_256_kernel<OUT, GATED, NATIVE><<<static_cast<unsigned>(g.tiles_m) * g.tiles_n, 512, kLds, st>>>(g, go);
+    gemm_fp8_256_kernel<OUT, ACT, NATIVE><<<static_cast<unsigned>(g.tiles_m) * g.tiles_n, 512, kLds, st>>>(g, go);
     return check_launch("gemm_fp8_256_kernel");
 }
 
@@ -573,7 +638,7 @@ Fp8Args make_args(const uint8_t* x, const float* xs, const uint8_t* w, const flo
 
 template <int OUT>
 int run_product(const Fp8Args& g, const Fp8Plan& plan, hipStream_t st) {
-    if (plan.big) return launch_big<OUT, false, OUT != MIQ_F32>(g, {}, st);
+    if (plan.big) return launch_big<OUT, kNoAct, OUT != MIQ_F32>(g, {}, st);
     return launch_tiles<OUT>(g, 1, st);
 }
 
@@ -627,13 +692,17 @@ extern "C" int miq_gated_fp8(const uint8_t* x, const float* x_scale, const uint8
     char* at = static_cast<char*>(workspace);
     Fp8Args g = make_args(x, x_scale, w_gate, gate_scale, w_up, up_scale, M, N, K, at, st);
     const Fp8Plan plan = make_plan(M, N, K, true);
-    if (plan.big) return launch_big<MIQ_F32, true, false>(g, {q, scale, act}, st);
+    if (plan.big)
+        return act == MIQ_ACT_SILU ? launch_big<MIQ_F32, MIQ_ACT_SILU, false>(g, {q, scale}, st)
+                                   : launch_big<MIQ_F32, MIQ_ACT_GELU, false>(g, {q, scale}, st);
     const int nblocks = static_cast<int>(ceil_div(N, 128));
     MIQ_REQUIRE(ceil_div(M * nblocks, 16) < (1ll << 24), MIQ_ERANGE, "miq_gated_fp8: too many blocks");
     g.out = at;
     g.kt_per_split = g.kblocks > 0 ? g.kblocks : 1;
     if (int rc = launch_tiles<MIQ_F32>(g, 2, st)) return rc;
-    gated_join_kernel<<<static_cast<unsigned>(ceil_div(M * nblocks, 16)), 256, 0, st>>>(reinterpret_cast<const float*>(at), 1, M, g.N,
-                                                                                     nblocks, act, q, scale);
+    const unsigned join = static_cast<unsigned>(ceil_div(M * nblocks, 16));
+    const float* slabs = reinterpret_cast<const float*>(at);
+    if (act == MIQ_ACT_SILU) gated_join_kernel<MIQ_ACT_SILU><<<join, 256, 0, st>>>(slabs, 1, M, g.N, nblocks, q, scale);
+    else gated_join_kernel<MIQ_ACT_GELU><<<join, 256, 0, st>>>(slabs, 1, M, g.N, nblocks, q, scale);
     return check_launch("gated_join_kernel");
 }
