@@ -38,31 +38,30 @@ struct Codes {
     v4i c[2];
 };
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+// The same fragment widened to bf16: h[i] is the operand of the i-th of a block's four matrix instructions.
 struct Widened {
-    v8bf h[4];
+    v4i h[4];
 };
+// Dword `pos` (0 .. 15) of a widened fragment: two codes.
+__device__ __forceinline__ void widen1(Widened& w, const Codes& f, int pos) {
+    const int src = f.c[pos >> 3][(pos & 7) >> 1];
+    w.h[pos >> 2][pos & 3] = (pos & 1) ? __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, 1.0f, true))
+                                       : __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, 1.0f, false));
+}
 __device__ __forceinline__ Widened widen(const Codes& f) {
     Widened r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int d = 0; d < 2; ++d) {
-            const int src = f.c[i >> 1][(i & 1) * 2 + d];
-            const v2bf lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, 1.0f, false);
-            const v2bf hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, 1.0f, true);
-            r.h[i][4 * d] = lo[0];
-            r.h[i][4 * d + 1] = lo[1];
-            r.h[i][4 * d + 2] = hi[0];
-            r.h[i][4 * d + 3] = hi[1];
-        }
+    for (int i = 0; i < 16; ++i) widen1(r, f, i);
     return r;
+}
+__device__ __forceinline__ v4f mfma_bf16(v4i w, v4i x, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w), __builtin_bit_cast(v8bf, x), c, 0, 0, 0);
 }
 // The products of one block, summed from zero.
 __device__ __forceinline__ v4f block_sum(const Widened& w, const Widened& x) {
     v4f c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.h[i], x.h[i], c, 0, 0, 0);
+    for (int i = 0; i < 4; ++i) c = mfma_bf16(w.h[i], x.h[i], c);
     return c;
 }
 
@@ -78,18 +77,26 @@ __device__ __forceinline__ void store_value(void* out, int64_t i, float v) {
     else static_cast<uint16_t*>(out)[i] = f32_to_bf16_bits(v);
 }
 
+// Four outputs of a 16-bit type.
+template <int OUT>
+__device__ __forceinline__ uint2 pack4(v4f v) {
+    if constexpr (OUT == MIQ_F16) {
+        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+        return __builtin_bit_cast(uint2, h4{static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1]), static_cast<_Float16>(v[2]),
+                                            static_cast<_Float16>(v[3])});
+    } else {
+        return pack4_bf16(v[0], v[1], v[2], v[3]);
+    }
+}
+
 // Four consecutive outputs of one row, `n` of them inside it.  `vec`: their address is aligned to four elements.
 template <int OUT>
 __device__ __forceinline__ void store4(void* out, int64_t i, int n, bool vec, v4f v) {
     if (vec && n >= 4) {
         if constexpr (OUT == MIQ_F32) {
             *reinterpret_cast<v4f*>(static_cast<float*>(out) + i) = v;
-        } else if constexpr (OUT == MIQ_F16) {
-            typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-            *reinterpret_cast<h4*>(static_cast<_Float16*>(out) + i) =
-                h4{static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1]), static_cast<_Float16>(v[2]), static_cast<_Float16>(v[3])};
         } else {
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i) = pack4_bf16(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i) = pack4<OUT>(v);
         }
     } else {
 #pragma unroll
@@ -132,11 +139,21 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* __restrict
     }
 }
 
-// The gate's activation, with the exponential and the error function in full fp32.
+// The gate's activation.  The logistic function is the hardware's power of two and reciprocal (one unit each): the rounded
+// argument of a large exponent costs its result some units, where the result is far below 1 and is multiplied by the gate,
+// so that the activation is within a few units of the gate's own size.  (With the library's exponential and an IEEE
+// division the epilogue of a 256 x 128 tile took 11 us of vector instructions, a tenth of a K of 4096.)
 template <int ACT>
 __device__ __forceinline__ float gate_value(float g) {
-    if constexpr (ACT == MIQ_ACT_SILU) return __fdiv_rn(g, 1.0f + expf(-g));
+    if constexpr (ACT == MIQ_ACT_SILU) return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504f));
     return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+}
+
+// What a wave's lanes wrote to LDS before this they may read after it (a wave's LDS operations are done in order).
+__device__ __forceinline__ void wave_lds_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
 }
 
 // BM x BN outputs a workgroup, two K-tile buffers, one barrier a K-tile.
@@ -223,9 +240,9 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
 // ---- 256 x 256 outputs a workgroup: large products -----------------------------------------------------------------
 // Eight waves, 2 (rows) x 4 (columns), a wave owns 128 x 64 outputs: eight row fragments by four column fragments.
 //
-// Within a K-tile a wave keeps the four column fragments and walks its row fragments; the sums of row fragment i - 1 are
-// scaled into the accumulators between the first matrix instructions of row fragment i, so that the vector work (the
-// scaling, and the widening of codes) runs in the shadow of the matrix pipe without a second set of sums.
+// Within a K-tile a wave keeps the four column fragments and walks its row fragments; the sums of an earlier fragment are
+// scaled into their accumulators behind the matrix instructions of a later one (two instructions later for the 8-bit form,
+// four chains later for the bf16 form), so that vector and matrix work overlap without waiting for each other.
 //
 // A K-tile is two phases, A (read and widen the column fragments, row fragments 0-3) and B (4-7), a barrier before each.
 // Waves 4-7, the second wave of every SIMD, run one phase behind waves 0-3: while one wave reads and widens its column
@@ -251,13 +268,10 @@ struct BigTypes<false> {
 };
 
 typedef int v8i __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ v4f first_mfma(const Codes& w, const Codes& x) {
+__device__ __forceinline__ v4f block_sum(const Codes& w, const Codes& x) {
     const v8i a = __builtin_shufflevector(w.c[0], w.c[1], 0, 1, 2, 3, 4, 5, 6, 7);
     const v8i b = __builtin_shufflevector(x.c[0], x.c[1], 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-}
-__device__ __forceinline__ v4f first_mfma(const Widened& w, const Widened& x) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.h[0], x.h[0], v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 }
 template <bool NATIVE>
 __device__ __forceinline__ auto operand(const Codes& c) {
@@ -271,19 +285,20 @@ struct GatedOut {
     float* scale;    // [ceil(N / 128), M]
 };
 
-template <int OUT, int ACT, bool NATIVE>
+template <int OUT, int ACT, bool NATIVE, int RF>
 __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut go) {
     constexpr bool GATED = ACT != kNoAct;
-    constexpr int kSlot = 256 * kTileK, kCols = GATED ? 128 : 256;
+    constexpr int kSlot = 256 * kTileK, kCols = GATED ? 128 : 256, kRows = RF * 32;   // (RF: row fragments of a wave)
+    constexpr int AS = RF / 2;   // row fragments of phase A
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 2, wn = wave & 3;
     int tm, tn;
     tile_coords(blockIdx.x, gridDim.x, g.tiles_m, g.tiles_n, 8, tm, tn);
-    const int64_t m0 = static_cast<int64_t>(tm) * 256;
+    const int64_t m0 = static_cast<int64_t>(tm) * kRows;
     const int n0 = tn * kCols;
-    const int mrows = static_cast<int>(g.M - m0 < 256 ? g.M - m0 : 256), nrows = g.N - n0 < kCols ? g.N - n0 : kCols;
+    const int mrows = static_cast<int>(g.M - m0 < kRows ? g.M - m0 : kRows), nrows = g.N - n0 < kCols ? g.N - n0 : kCols;
 
     // Staging: a wave-instruction moves 8 rows x 128 B; wave v moves rows v * 8 + 64 i, i = 0 .. 3, of each operand.  K-tile
     // and row group advance in the descriptor (scalar registers); a lane's offset stays.  Rows past the matrix lie past the
@@ -316,7 +331,7 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
     // 16-lane rows between two copies.  Rows past the end read as 0.
     auto row_scales = [&](int kt, int half) {
         const __amdgpu_buffer_rsrc_t rs = make_rsrc(g.xs + static_cast<int64_t>(kt) * g.M + m0, static_cast<uint32_t>(mrows) * 4);
-        return __builtin_amdgcn_raw_buffer_load_b32(rs, static_cast<uint32_t>(wm * 128 + half * 64 + lane) * 4, 0, 0);
+        return __builtin_amdgcn_raw_buffer_load_b32(rs, static_cast<uint32_t>(wm * (RF * 16) + half * 64 + lane) * 4, 0, 0);
     };
     auto spread = [&](uint32_t v, float (&s)[4]) {
         const auto halves = __builtin_amdgcn_permlane32_swap(v, v, false, false);
@@ -342,33 +357,50 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
     };
 
     using Frag = typename BigTypes<NATIVE>::Frag;
-    v4f acc[8][4] = {};
-    v4f c[4] = {};
-    float s_cur[4], s_last0 = 0.f, s_last1 = 0.f;   // s_last: the scales of the sums still in c (row fragment 7 of the tile before)
+    v4f acc[RF][4] = {};
+    v4f c[4] = {};   // sums of a block that are not scaled yet
+    float s_cur[4], s[2] = {}, s_old[2] = {};   // scales of this row fragment (gate's or only, up's) and of the one before
     const int nt = g.kblocks;
-    Frag wf[4];
-    Codes raw;
+    Frag wf[4], xf[2];        // column fragments; row fragment i (8-bit: in xf[i & 1], read one step ahead)
+    Codes raw;                // the codes of row fragment i + 1
+    auto scale_in = [&](v4f& a, const v4f& sum, float by, int e) { a[e] = __builtin_fmaf(sum[e], by, a[e]); };
+    auto pin = [](v4f& a) { asm volatile("" : "+v"(a)); };   // scaled here, and not where the loop ends
     auto rows_step = [&](auto step, int xt, uint32_t sv, float sw0, float sw1) {
-        constexpr int i = decltype(step)::value;
-        const Frag xf = operand<NATIVE>(raw);
-        if (i < 7) raw = read(xt, (i + 1) * 16);
-        const int p = i ? i - 1 : 7;   // the row fragment whose sums are in c
+        constexpr int i = decltype(step)::value, p = i ? i - 1 : RF - 1;   // p: the row fragment before
+        if constexpr (i % 4 == 0) spread(sv, s_cur);
+        s_old[0] = s[0];
+        s_old[1] = s[1];
+        s[0] = s_cur[i % 4] * sw0;   // of column fragments 0, 1
+        s[1] = GATED ? s_cur[i % 4] * sw1 : s[0];
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (NATIVE) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            add_scaled(acc[p][j], c[j], GATED && j >= 2 ? s_last1 : s_last0);
-            asm volatile("" : "+v"(acc[p][j]));   // here and not at the loop's end, with all sums kept until then
-            c[j] = first_mfma(wf[j], xf);
-        }
-        if constexpr (!NATIVE) {
+            for (int j = 0; j < 4; ++j) {
+                c[j] = block_sum(wf[j], xf[i & 1]);
+                // column fragment j - 2 of this row fragment, or j + 2 of the one before
+                v4f& a = j < 2 ? acc[p][j + 2] : acc[i][j - 2];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) scale_in(a, c[j ^ 2], j < 2 ? s_old[0] : s[0], e);
+                pin(a);
+                if (i < RF - 1 && j == 0) xf[(i + 1) & 1] = read(xt, (i + 1) * 16);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            if (i > 0) xf[0] = widen(raw);
+            if (i < RF - 1) raw = read(xt, (i + 1) * 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) scale_in(acc[p][j], c[j], s_old[j >> 1], e);
+                pin(acc[p][j]);
+                c[j] = mfma_bf16(wf[j].h[0], xf[0].h[0], v4f{0.f, 0.f, 0.f, 0.f});
+            }
 #pragma unroll
             for (int h = 1; h < 4; ++h)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) c[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j].h[h], xf.h[h], c[j], 0, 0, 0);
+                for (int j = 0; j < 4; ++j) c[j] = mfma_bf16(wf[j].h[h], xf[0].h[h], c[j]);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (i % 4 == 0) spread(sv, s_cur);
-        s_last0 = s_cur[i % 4] * sw0;
-        if constexpr (GATED) s_last1 = s_cur[i % 4] * sw1;
-        __builtin_amdgcn_sched_barrier(0);
     };
     auto barrier = [&] {
         asm volatile("" ::: "memory");
@@ -391,41 +423,49 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
         int slot = 0;   // of x(t)
         for (int t = 0; t < nt; ++t) {
             asm volatile("" : "+s"(group));   // (one loop for both groups: the body is not worth duplicating)
-            const int xt = x_slot(slot) + wm * 128 * kTileK, wt = w_slot(t);
+            const int xt = x_slot(slot) + wm * (RF * 16) * kTileK, wt = w_slot(t);
             const int ahead = slot == 0 ? 2 : slot - 1;   // of x(t + 2), and of x(t - 1)
             slot = slot == 2 ? 0 : slot + 1;
             const float sw0 = ws0[t], sw1 = GATED ? ws1[t] : sw0;
             // phase A
             stage(group == 0, group ? t + 2 : t + 1, group ? x_slot(ahead) : w_slot(t + 1));
-            raw = read(xt, 0);
+            xf[0] = operand<NATIVE>(read(xt, 0));
 #pragma unroll
             for (int j = 0; j < 4; ++j) wf[j] = operand<NATIVE>(read(wt, w_row(j)));
             rows_step(integral_constant<int, 0>{}, xt, sv0, sw0, sw1);
             rows_step(integral_constant<int, 1>{}, xt, sv0, sw0, sw1);
-            rows_step(integral_constant<int, 2>{}, xt, sv0, sw0, sw1);
-            rows_step(integral_constant<int, 3>{}, xt, sv0, sw0, sw1);
+            if constexpr (AS > 2) rows_step(integral_constant<int, 2>{}, xt, sv0, sw0, sw1);
+            if constexpr (AS > 3) rows_step(integral_constant<int, 3>{}, xt, sv0, sw0, sw1);
             if (group) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");   // x(t + 1), w(t + 1); x(t + 2) stays in flight
             barrier();
             // phase B
             stage(group != 0, t + 2, group ? w_slot(t + 2) : x_slot(ahead));
             const int tn1 = t + 1 < nt ? t + 1 : t;
             sv0 = row_scales(tn1, 0);
+            const uint32_t sv1_next = row_scales(tn1, 1);
+            if constexpr (AS < 3) rows_step(integral_constant<int, 2>{}, xt, sv1, sw0, sw1);
+            if constexpr (AS < 4) rows_step(integral_constant<int, 3>{}, xt, sv1, sw0, sw1);
             rows_step(integral_constant<int, 4>{}, xt, sv1, sw0, sw1);
-            sv1 = row_scales(tn1, 1);
             rows_step(integral_constant<int, 5>{}, xt, sv1, sw0, sw1);
-            rows_step(integral_constant<int, 6>{}, xt, sv1, sw0, sw1);
-            rows_step(integral_constant<int, 7>{}, xt, sv1, sw0, sw1);
+            if constexpr (RF == 8) {
+                rows_step(integral_constant<int, 6>{}, xt, sv1, sw0, sw1);
+                rows_step(integral_constant<int, 7>{}, xt, sv1, sw0, sw1);
+            }
+            sv1 = sv1_next;
             if (!group) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
             barrier();
         }
         if (wm == 0) barrier();   // every wave executes the same number of barriers
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the pieces requested for K-tiles past the end
     }
+    // the sums still waiting
 #pragma unroll
-    for (int j = 0; j < 4; ++j) add_scaled(acc[7][j], c[j], GATED && j >= 2 ? s_last1 : s_last0);
+    for (int j = NATIVE ? 2 : 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) scale_in(acc[RF - 1][j], c[j], s[j >> 1], e);
 
     // Results of a fragment: 4 * (lane >> 4) + register -> column, lane & 15 -> row.
-    const int64_t mw = m0 + wm * 128 + (lane & 15);
+    const int64_t mw = m0 + wm * (RF * 16) + (lane & 15);
     if constexpr (GATED) {
         // The tile's 128 columns are a block of the result.  Its maximum for each row: over the lane's eight values, the
         // four lanes of the row, and the four waves of the row through LDS.
@@ -444,10 +484,10 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
             top = o > top ? o : top;
             o = __shfl_xor(top, 32, 64);
             top = o > top ? o : top;
-            if (lane < 16) tops[wn * 256 + wm * 128 + i * 16 + lane] = top;
+            if (lane < 16) tops[wn * 256 + wm * (RF * 16) + i * 16 + lane] = top;
         };
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < RF; ++i) {
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -456,7 +496,7 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
         }
         __syncthreads();
         auto row_top = [&](int i) {
-            const uint32_t* t = tops + wm * 128 + i * 16 + (lane & 15);
+            const uint32_t* t = tops + wm * (RF * 16) + i * 16 + (lane & 15);
             uint32_t top = t[0];
 #pragma unroll
             for (int w = 1; w < 4; ++w) top = t[w * 256] > top ? t[w * 256] : top;
@@ -464,17 +504,17 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
         };
         bool spoiled = false;   // some value of this wave's rows is not finite: the same in the four waves of these rows
 #pragma unroll
-        for (int i = 0; i < 8; ++i) spoiled |= row_top(i) >= kInfBits;
+        for (int i = 0; i < RF; ++i) spoiled |= row_top(i) >= kInfBits;
         spoiled = __any(spoiled);
         __syncthreads();
         if (spoiled) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top_of(i, finite_magnitude_bits);
+            for (int i = 0; i < RF; ++i) top_of(i, finite_magnitude_bits);
         }
         __syncthreads();
         const bool vec = (g.N & 3) == 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < RF; ++i) {
             const int64_t m = mw + i * 16;
             const BlockScale s = block_scale(row_top(i));
             if (m >= g.M) continue;
@@ -494,19 +534,69 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
             }
         }
     } else {
-        const bool vec = (g.N & 3) == 0;
+        __syncthreads();               // every wave has read its last K-tile (LDS is used again below)
+        const int nw = n0 + wn * 64;   // the wave's 64 columns
+        if (g.bias) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int n = n0 + wn * 64 + j * 16 + (lane >> 4) * 4;
-            if (n >= g.N) continue;
-            v4f b = {0.f, 0.f, 0.f, 0.f};
-            if (g.bias)
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < g.N) b[e] = g.bias[n + e];
+            for (int j = 0; j < 4; ++j) {
+                const int n = nw + j * 16 + (lane >> 4) * 4;
+                v4f b;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int64_t m = mw + i * 16;
-                if (m < g.M) store4<OUT>(g.out, m * g.N + n, g.N - n, vec, acc[i][j] + b);
+                for (int e = 0; e < 4; ++e) b[e] = n + e < g.N ? g.bias[n + e] : 0.f;
+#pragma unroll
+                for (int i = 0; i < RF; ++i) acc[i][j] += b;
+            }
+        }
+        if ((g.N & 7) == 0 && nw + 64 <= g.N) {
+            // Whole cache lines: as they lie, an instruction would write sixteen rows x 64 (fp32) or 32 bytes.  Lanes r and
+            // r ^ 8 of a 16-lane row trade halves of a row's pieces, so that one writes eight rows x 128 bytes.
+            const int r = lane & 15;
+            const bool lo = r < 8;
+            auto store_rows = [&](v4i first, v4i second, int64_t m1, int n, int size) {   // first: columns of the low half
+                v4i a, b;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int recv = __builtin_amdgcn_update_dpp(0, lo ? second[e] : first[e], 0x128 /* row_ror:8 */, 0xf, 0xf, false);
+                    a[e] = lo ? first[e] : recv;
+                    b[e] = lo ? recv : second[e];
+                }
+                char* o = static_cast<char*>(g.out) + (m1 * g.N + n) * size;
+                if (m1 < g.M) __builtin_nontemporal_store(a, reinterpret_cast<v4i*>(o));
+                if (m1 + 8 < g.M) __builtin_nontemporal_store(b, reinterpret_cast<v4i*>(o + 8ll * g.N * size));
+            };
+#pragma unroll
+            for (int i = 0; i < RF; ++i) {
+                const int64_t m1 = m0 + wm * (RF * 16) + i * 16 + (r & 7);
+                if constexpr (OUT == MIQ_F32) {
+#pragma unroll
+                    for (int j = 0; j < 4; j += 2)
+                        store_rows(__builtin_bit_cast(v4i, acc[i][j]), __builtin_bit_cast(v4i, acc[i][j + 1]), m1,
+                                   nw + j * 16 + (lo ? 0 : 16) + (lane >> 4) * 4, 4);
+                } else {
+                    uint2 p[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) p[j] = pack4<OUT>(acc[i][j]);
+                    store_rows(pair_rows_bf16(p[0], p[1]), pair_rows_bf16(p[2], p[3]), m1, nw + (lo ? 0 : 32) + paired_offset(lane), 2);
+                }
+            }
+        } else {
+            // Rows that start anywhere: a row fragment's 16 x 64 through LDS (the wave's own 16 rows of 68 floats), then one row
+            // an instruction, a column a lane.
+            float* const rows = reinterpret_cast<float*>(smem) + wave * (16 * 68);
+            const int n = nw + lane;
+#pragma unroll
+            for (int i = 0; i < RF; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) *reinterpret_cast<v4f*>(rows + (lane & 15) * 68 + j * 16 + (lane >> 4) * 4) = acc[i][j];
+                wave_lds_order();
+                const int64_t m = m0 + wm * (RF * 16) + i * 16;
+                float v[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) v[r] = rows[r * 68 + lane];
+                wave_lds_order();
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (n < g.N && m + r < g.M) store_value<OUT>(g.out, (m + r) * g.N + n, v[r]);
             }
         }
     }
@@ -571,16 +661,23 @@ const uint8_t* pad_rows(const uint8_t* src, int64_t rows, int64_t K, char*& at, 
 
 // What a product is cut into: which kernel, and how much workspace it needs behind the padded operands.
 struct Fp8Plan {
-    bool big;        // 256 x 256 tiles
+    int big;         // rows of the large kernel's tile, 256 or 192; 0: the tile kernel
     size_t slabs;    // bytes
 };
 
 // Large products: at least this many 256 x 256 tiles run on the 256 x 256 kernel.
 constexpr int64_t kBigTiles = 128;
+constexpr int64_t kCus = 256;
 
 Fp8Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
     Fp8Plan p{};
-    p.big = M > 128 && ceil_div(M, 256) * ceil_div(N, gated ? 128 : 256) >= kBigTiles;
+    const int64_t across = ceil_div(N, gated ? 128 : 256);
+    if (M > 128 && ceil_div(M, 256) * across >= kBigTiles) {
+        // One workgroup a CU: a launch takes as many rounds as its tiles need.  A 192-row tile takes 5/6 of the time of a
+        // 256-row one (1000 x 10001 x 4000 fp32: 104 us in one round of 240 tiles, 123 us in one of 160).
+        const int64_t r256 = ceil_div(ceil_div(M, 256) * across, kCus), r192 = ceil_div(ceil_div(M, 192) * across, kCus);
+        p.big = 6 * r256 <= 5 * r192 ? 256 : 192;
+    }
     if (gated && !p.big) p.slabs = static_cast<size_t>(2 * 4 * M * N);
     return p;
 }
@@ -595,15 +692,19 @@ int launch_tiles(Fp8Args g, int products, hipStream_t st) {
     return check_launch("gemm_fp8_tile_kernel");
 }
 
-template <int OUT, int ACT, bool NATIVE>
-int launch_big(Fp8Args g, GatedOut go, hipStream_t st) {
+template <int OUT, int ACT, bool NATIVE, int RF>
+int launch_big_rows(Fp8Args g, GatedOut go, hipStream_t st) {
     constexpr int kLds = 5 * 256 * kTileK;
-    g.tiles_m = static_cast<int>(ceil_div(g.M, 256));
+    g.tiles_m = static_cast<int>(ceil_div(g.M, RF * 32));
     g.tiles_n = static_cast<int>(ceil_div(g.N, ACT != kNoAct ? 128 : 256));
-    const void* fn = reinterpret_cast<const void*>(&gemm_fp8_256_kernel<OUT, ACT, NATIVE>);
+    const void* fn = reinterpret_cast<const void*>(&gemm_fp8_256_kernel<OUT, ACT, NATIVE, RF>);
     if (int rc = allow_lds(fn, kLds)) return rc;
-    gemm_fp8_256_kernel<OUT, ACT, NATIVE><<<static_cast<unsigned>(g.tiles_m) * g.tiles_n, 512, kLds, st>>>(g, go);
+    gemm_fp8_256_kernel<OUT, ACT, NATIVE, RF><<<static_cast<unsigned>(g.tiles_m) * g.tiles_n, 512, kLds, st>>>(g, go);
     return check_launch("gemm_fp8_256_kernel");
+}
+template <int OUT, int ACT, bool NATIVE>
+int launch_big(const Fp8Plan& plan, const Fp8Args& g, GatedOut go, hipStream_t st) {
+    return plan.big == 256 ? launch_big_rows<OUT, ACT, NATIVE, 8>(g, go, st) : launch_big_rows<OUT, ACT, NATIVE, 6>(g, go, st);
 }
 
 // Checks that both products share; `weights` of them, 1 or 2.
@@ -638,7 +739,7 @@ Fp8Args make_args(const uint8_t* x, const float* xs, const uint8_t* w, const flo
 
 template <int OUT>
 int run_product(const Fp8Args& g, const Fp8Plan& plan, hipStream_t st) {
-    if (plan.big) return launch_big<OUT, kNoAct, OUT != MIQ_F32>(g, {}, st);
+    if (plan.big) return launch_big<OUT, kNoAct, OUT != MIQ_F32>(plan, g, {}, st);
     return launch_tiles<OUT>(g, 1, st);
 }
 
@@ -693,8 +794,8 @@ extern "C" int miq_gated_fp8(const uint8_t* x, const float* x_scale, const uint8
     Fp8Args g = make_args(x, x_scale, w_gate, gate_scale, w_up, up_scale, M, N, K, at, st);
     const Fp8Plan plan = make_plan(M, N, K, true);
     if (plan.big)
-        return act == MIQ_ACT_SILU ? launch_big<MIQ_F32, MIQ_ACT_SILU, false>(g, {q, scale}, st)
-                                   : launch_big<MIQ_F32, MIQ_ACT_GELU, false>(g, {q, scale}, st);
+        return act == MIQ_ACT_SILU ? launch_big<MIQ_F32, MIQ_ACT_SILU, false>(plan, g, {q, scale}, st)
+                                   : launch_big<MIQ_F32, MIQ_ACT_GELU, false>(plan, g, {q, scale}, st);
     const int nblocks = static_cast<int>(ceil_div(N, 128));
     MIQ_REQUIRE(ceil_div(M * nblocks, 16) < (1ll << 24), MIQ_ERANGE, "miq_gated_fp8: too many blocks");
     g.out = at;
