@@ -65,6 +65,32 @@ __device__ __forceinline__ v4f block_sum(const Widened& w, const Widened& x) {
     return c;
 }
 
+// The operand of a fragment: the codes themselves for the 8-bit instruction (NATIVE), else widened.
+template <bool NATIVE>
+struct OperandOf;
+template <>
+struct OperandOf<true> {
+    using Frag = Codes;
+};
+template <>
+struct OperandOf<false> {
+    using Frag = Widened;
+};
+
+constexpr int kNoAct = -1;   // (an epilogue without a gate)
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ v4f block_sum(const Codes& w, const Codes& x) {
+    const v8i a = __builtin_shufflevector(w.c[0], w.c[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    const v8i b = __builtin_shufflevector(x.c[0], x.c[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+template <bool NATIVE>
+__device__ __forceinline__ auto operand(const Codes& c) {
+    if constexpr (NATIVE) return c;
+    else return widen(c);
+}
+
 __device__ __forceinline__ void add_scaled(v4f& acc, v4f c, float s) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(c[e], s, acc[e]);
@@ -156,13 +182,21 @@ __device__ __forceinline__ void wave_lds_order() {
     asm volatile("" ::: "memory");
 }
 
-// BM x BN outputs a workgroup, two K-tile buffers, one barrier a K-tile.
-template <int BM, int BN, int WAVES_M, int WAVES_N, int OUT>
+// ---- small tiles: products that do not fill the chip with 256 x 256 ones --------------------------------------------
+// BM x BN outputs a workgroup.  STAGES == 2: two K-tile buffers and one barrier a K-tile, for tiles whose matrix work covers
+// a fetch; STAGES > 2: a ring with STAGES - 1 K-tiles in flight and a counted wait, for the thin ones (a few rows against a
+// weight that streams from HBM), whose K-tile of matrix work is far shorter than a fetch.  Split-K: slice blockIdx.y sums its
+// K-tiles into an fp32 slab of its own; blockIdx.z picks the weight of a gated product.
+constexpr int tile_stage_bytes(int bm, int bn, int waves) { return (bm + bn) * kTileK + waves * ((bm + 63) / 64) * 256; }
+
+template <int BM, int BN, int WAVES_M, int WAVES_N, int STAGES, int OUT, bool NATIVE>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(Fp8Args g) {
     constexpr int NWAVES = WAVES_M * WAVES_N;
     constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, FM = WM / 16, FN = WN / 16;
-    constexpr int STAGE = (BM + BN) * kTileK;
+    constexpr int kRowBytes = (BM + BN) * kTileK, kScaleLoads = (BM + 63) / 64;
+    constexpr int STAGE = tile_stage_bytes(BM, BN, NWAVES);
     static_assert(128 % BN == 0, "a tile's columns lie in one 128-row block of the weight");
+    static_assert((BM / 8) % NWAVES == 0 && (BN / 8) % NWAVES == 0, "every wave issues the same number of pieces");
     extern __shared__ __attribute__((aligned(16))) char smem[];
 
     const int lane = threadIdx.x & 63;
@@ -176,7 +210,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
     const int mrows = static_cast<int>(g.M - m0 < BM ? g.M - m0 : BM), nrows = g.N - n0 < BN ? g.N - n0 : BN;
     const uint8_t* xrows = g.x + m0 * g.K;
     const uint8_t* wrows = g.w[which] + static_cast<int64_t>(n0) * g.K;
-    const float* wscale = g.ws[which] + static_cast<int64_t>(n0 / 128) * g.kblocks;
+    using scalar_floats = const __attribute__((address_space(4))) float*;   // (read through the scalar unit)
+    const scalar_floats wscale = (scalar_floats)(g.ws[which] + static_cast<int64_t>(n0 / 128) * g.kblocks);
 
     const int kt0 = g.kt_per_split ? static_cast<int>(blockIdx.y) * g.kt_per_split : 0;
     const int kt1 = g.kt_per_split && kt0 + g.kt_per_split < g.kblocks ? kt0 + g.kt_per_split : g.kblocks;
@@ -187,36 +222,63 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
 
     v4f acc[FM][FN] = {};
     const int lo0 = frag_lane_offset(lane, 0), lo1 = frag_lane_offset(lane, 1);
-    int64_t row[FM];   // this lane's rows, held inside the matrix for the scales' loads
+    // A stage of LDS: BM + BN rows of a K-tile, and for each wave a copy of the rows' scales (fetched by LDS-DMA like the rows:
+    // a scale loaded into a register would be waited for together with the younger rows' requests).
+    auto stage = [&](char* buf, int kt) {   // (a K-tile past the slice is requested out of range: zeros, no memory traffic)
+        const int k = kt < kt1 ? kt : g.kblocks;
+        stage_rows<BM, NWAVES>(xrows, mrows, g.K, k, buf, wave, lane);
+        stage_rows<BN, NWAVES>(wrows, nrows, g.K, k, buf + BM * kTileK, wave, lane);
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(g.xs + static_cast<int64_t>(kt < kt1 ? kt : kt0) * g.M + m0, static_cast<uint32_t>(mrows) * 4);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int64_t m = m0 + wm * WM + i * 16 + (lane & 15);
-        row[i] = m < g.M ? m : g.M - 1;
-    }
-    auto stage = [&](int kt) {
-        char* buf = smem + (kt & 1) * STAGE;
-        stage_rows<BM, NWAVES>(xrows, mrows, g.K, kt, buf, wave, lane);
-        stage_rows<BN, NWAVES>(wrows, nrows, g.K, kt, buf + BM * kTileK, wave, lane);
+        for (int i = 0; i < kScaleLoads; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(buf + kRowBytes + (wave * kScaleLoads + i) * 256), 4,
+                                                     static_cast<uint32_t>(i * 64 + lane) * 4, 0, 0, 0);
     };
-    if (kt0 < kt1) stage(kt0);
-    __syncthreads();
-    for (int kt = kt0; kt < kt1; ++kt) {
-        if (kt + 1 < kt1) stage(kt + 1);
-        const char* xt = smem + (kt & 1) * STAGE + wm * WM * kTileK;
-        const char* wt = smem + (kt & 1) * STAGE + (BM + wn * WN) * kTileK;
-        float s[FM];
-        Widened xf[FM], wf[FN];
+    auto multiply = [&](const char* buf, int kt) {
+        const float* xs = reinterpret_cast<const float*>(buf + kRowBytes + wave * kScaleLoads * 256) + wm * WM + (lane & 15);
+        const char* xt = buf + wm * WM * kTileK;
+        const char* wt = buf + (BM + wn * WN) * kTileK;
+        const float sw = wscale[kt];
+        typename OperandOf<NATIVE>::Frag wf[FN];
 #pragma unroll
-        for (int i = 0; i < FM; ++i) s[i] = g.xs[static_cast<int64_t>(kt) * g.M + row[i]] * wscale[kt];
+        for (int j = 0; j < FN; ++j)
+            wf[j] = operand<NATIVE>({{lds_read16(wt + j * 16 * kTileK + lo0), lds_read16(wt + j * 16 * kTileK + lo1)}});
 #pragma unroll
-        for (int i = 0; i < FM; ++i) xf[i] = widen({{lds_read16(xt + i * 16 * kTileK + lo0), lds_read16(xt + i * 16 * kTileK + lo1)}});
+        for (int i = 0; i < FM; ++i) {
+            const auto xf = operand<NATIVE>(Codes{{lds_read16(xt + i * 16 * kTileK + lo0), lds_read16(xt + i * 16 * kTileK + lo1)}});
+            const float s = xs[i * 16] * sw;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) wf[j] = widen({{lds_read16(wt + j * 16 * kTileK + lo0), lds_read16(wt + j * 16 * kTileK + lo1)}});
+            for (int j = 0; j < FN; ++j) add_scaled(acc[i][j], block_sum(wf[j], xf), s);
+        }
+    };
+
+    if (kt0 < kt1) {
+        if constexpr (STAGES == 2) {
+            stage(smem, kt0);
+            __syncthreads();
+            for (int kt = kt0; kt < kt1; ++kt) {
+                if (kt + 1 < kt1) stage(smem + ((kt + 1 - kt0) & 1) * STAGE, kt + 1);
+                multiply(smem + ((kt - kt0) & 1) * STAGE, kt);
+                __syncthreads();   // the next K-tile has landed and this one has been read
+            }
+        } else {
+            // All but the youngest STAGES - 2 K-tiles have landed when at most that many K-tiles' requests are outstanding.
+            constexpr int kKeep = ((BM / 8 + BN / 8) / NWAVES + kScaleLoads) * (STAGES - 2);
+            static_assert(kKeep <= 63, "vmcnt is a 6-bit counter");
 #pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) add_scaled(acc[i][j], block_sum(wf[j], xf[i]), s[i]);
-        __syncthreads();   // the next K-tile has landed and this one has been read
+            for (int t = 0; t < STAGES - 1; ++t) stage(smem + t * STAGE, kt0 + t);
+            int slot = 0, fill = STAGES - 1;
+            for (int kt = kt0; kt < kt1; ++kt) {
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kKeep) : "memory");
+                __builtin_amdgcn_s_barrier();   // K-tile kt is there for every wave; every wave has read kt - 1
+                asm volatile("" ::: "memory");
+                stage(smem + fill * STAGE, kt + STAGES - 1);
+                multiply(smem + slot * STAGE, kt);
+                slot = slot + 1 == STAGES ? 0 : slot + 1;
+                fill = fill + 1 == STAGES ? 0 : fill + 1;
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
     }
 
     // A fragment's results: 4 * (lane >> 4) + register -> column n, lane & 15 -> row m.
@@ -235,6 +297,110 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
             if (m < g.M) store4<OUT>(out, m * g.N + n, g.N - n, vec, acc[i][j] + b);
         }
     }
+}
+
+// out = the slabs' sum (in order) + bias
+template <int OUT>
+__global__ __launch_bounds__(256) void splitk_sum_kernel(const float* __restrict__ slabs, int splits, int64_t M, int N,
+                                                         const float* __restrict__ bias, void* __restrict__ out) {
+    const int64_t total = M * N;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+        float v = 0.f;
+        for (int s = 0; s < splits; ++s) v += slabs[s * total + i];
+        store_value<OUT>(out, i, bias ? v + bias[i % N] : v);
+    }
+}
+
+// ---- at most 16 rows: the weight streams once, HBM -> registers ------------------------------------------------------
+// A row group of 16 weight rows is one operand fragment, and nothing is shared between waves, so nothing is staged: a lane
+// loads the chunks that the instructions want from it.  A workgroup of eight waves owns GROUPS row groups; wave v sums the
+// K-tiles v, v + 8, ... (eight consecutive K-tiles are 1 KiB of a row), DEPTH of them in flight, and the eight partial sums
+// meet in LDS.  A gated product's groups are the gate's and the up projection's same 16 columns: the workgroup finishes
+// act(g) * u in fp32, and the quantizer follows.
+template <int GROUPS, int DEPTH, int OUT, int ACT>
+__global__ __launch_bounds__(512) void gemm_fp8_rows16_kernel(Fp8Args g) {
+    constexpr bool GATED = ACT != kNoAct;
+    static_assert(!GATED || GROUPS == 2, "a gate's group and an up projection's");
+    constexpr int kWaves = 8, kCols = GATED ? 16 : GROUPS * 16;
+    __shared__ float part[kWaves * GROUPS * 256];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * kCols;
+    const int nrows = g.N - n0 < kCols ? g.N - n0 : kCols;
+    const int kt0 = g.kt_per_split ? static_cast<int>(blockIdx.y) * g.kt_per_split : 0;
+    const int kt1 = g.kt_per_split && kt0 + g.kt_per_split < g.kblocks ? kt0 + g.kt_per_split : g.kblocks;
+
+    // Rows past the matrices lie past the descriptors' ends and read as zeros.
+    const int cb = (lane >> 4) * kChunk;
+    const uint32_t row = static_cast<uint32_t>(lane & 15) * static_cast<uint32_t>(g.K) + cb;
+    const __amdgpu_buffer_rsrc_t rx = make_rsrc(g.x, static_cast<uint32_t>(g.M) * static_cast<uint32_t>(g.K));
+    __amdgpu_buffer_rsrc_t rw[GROUPS];
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) {
+        const int first = GATED ? 0 : j * 16, left = nrows - first;
+        rw[j] = make_rsrc(g.w[GATED ? j : 0] + static_cast<int64_t>(n0 + first) * g.K,
+                          left > 0 ? static_cast<uint32_t>(left) * static_cast<uint32_t>(g.K) : 0);
+    }
+    using scalar_floats = const __attribute__((address_space(4))) float*;
+    scalar_floats wscale[GATED ? 2 : 1];
+#pragma unroll
+    for (int j = 0; j < (GATED ? 2 : 1); ++j) wscale[j] = (scalar_floats)(g.ws[j] + static_cast<int64_t>(n0 / 128) * g.kblocks);
+
+    struct Slot {
+        Codes w[GROUPS], x;
+        float s;   // the scale of row lane & 15
+    };
+    auto fill = [&](Slot& s, int kt) {
+        const bool in = kt < kt1;
+        const int kfirst = in ? kt * kTileK : 1 << 30;   // (past the slice: past K)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = kfirst + h * 64;
+            const uint32_t off = k + cb < g.K ? row + k : kOob;
+#pragma unroll
+            for (int j = 0; j < GROUPS; ++j) s.w[j].c[h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw[j], off, 0, 0));
+            s.x.c[h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 0, 0));
+        }
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(g.xs + static_cast<int64_t>(in ? kt : kt0) * g.M, static_cast<uint32_t>(g.M) * 4);
+        s.s = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, (lane & 15) * 4, 0, 0));
+    };
+
+    v4f acc[GROUPS] = {};
+    Slot ring[DEPTH];
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) fill(ring[u], kt0 + wave + u * kWaves);
+    for (int kt = kt0 + wave; kt < kt1; kt += kWaves * DEPTH) {
+#pragma unroll
+        for (int u = 0; u < DEPTH; ++u) {
+            const int t = kt + u * kWaves, ts = t < kt1 ? t : kt0;   // (a K-tile past the slice: zeros, times some scale)
+            const Widened x = widen(ring[u].x);
+#pragma unroll
+            for (int j = 0; j < GROUPS; ++j) add_scaled(acc[j], block_sum(widen(ring[u].w[j]), x), ring[u].s * wscale[GATED ? j : 0][ts]);
+            fill(ring[u], t + DEPTH * kWaves);
+        }
+    }
+
+    // A fragment's results: 4 * (lane >> 4) + register -> weight row, lane & 15 -> row m.
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) *reinterpret_cast<v4f*>(&part[((wave * GROUPS + j) * 64 + lane) * 4]) = acc[j];
+    __syncthreads();
+    auto sum_of = [&](int j, int m, int ch) {
+        const int at = (j * 64 + (ch >> 2) * 16 + m) * 4 + (ch & 3);
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) v += part[w * GROUPS * 256 + at];
+        return v;
+    };
+    const int e = threadIdx.x;
+    if (e >= 16 * kCols) return;
+    const int m = e / kCols, ch = e % kCols, n = n0 + ch;
+    if (m >= g.M || n >= g.N) return;
+    void* out = g.out;
+    if (g.kt_per_split) out = static_cast<float*>(out) + static_cast<int64_t>(blockIdx.y) * g.M * g.N;
+    float v;
+    if constexpr (GATED) v = gate_value<ACT>(sum_of(0, m, ch)) * sum_of(1, m, ch);
+    else v = sum_of(ch >> 4, m, ch & 15) + (g.bias && !g.kt_per_split ? g.bias[n] : 0.f);
+    store_value<OUT>(out, static_cast<int64_t>(m) * g.N + n, v);
 }
 
 // ---- 256 x 256 outputs a workgroup: large products -----------------------------------------------------------------
@@ -256,30 +422,6 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
 //
 // GATED: the tile is 128 columns of both weights, a wave's column fragments 0, 1 the gate's and 2, 3 the up projection's
 // same 32 columns, so that a lane holds both factors of its outputs and the 128 columns are one block of the result.
-template <bool NATIVE>
-struct BigTypes;
-template <>
-struct BigTypes<true> {
-    using Frag = Codes;
-};
-template <>
-struct BigTypes<false> {
-    using Frag = Widened;
-};
-
-typedef int v8i __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ v4f block_sum(const Codes& w, const Codes& x) {
-    const v8i a = __builtin_shufflevector(w.c[0], w.c[1], 0, 1, 2, 3, 4, 5, 6, 7);
-    const v8i b = __builtin_shufflevector(x.c[0], x.c[1], 0, 1, 2, 3, 4, 5, 6, 7);
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-}
-template <bool NATIVE>
-__device__ __forceinline__ auto operand(const Codes& c) {
-    if constexpr (NATIVE) return c;
-    else return widen(c);
-}
-
-constexpr int kNoAct = -1;
 struct GatedOut {
     uint8_t* q;      // [M, N]
     float* scale;    // [ceil(N / 128), M]
@@ -356,7 +498,7 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
         return Codes{{lds_read16(smem + tile + lo0 + row * kTileK), lds_read16(smem + tile + lo1 + row * kTileK)}};
     };
 
-    using Frag = typename BigTypes<NATIVE>::Frag;
+    using Frag = typename OperandOf<NATIVE>::Frag;
     v4f acc[RF][4] = {};
     v4f c[4] = {};   // sums of a block that are not scaled yet
     float s_cur[4], s[2] = {}, s_old[2] = {};   // scales of this row fragment (gate's or only, up's) and of the one before
@@ -659,10 +801,13 @@ const uint8_t* pad_rows(const uint8_t* src, int64_t rows, int64_t K, char*& at, 
     return dst;
 }
 
-// What a product is cut into: which kernel, and how much workspace it needs behind the padded operands.
+// What a product is cut into: which kernel, how K is split, and how much workspace that needs behind the padded operands.
 struct Fp8Plan {
-    int big;         // rows of the large kernel's tile, 256 or 192; 0: the tile kernel
-    size_t slabs;    // bytes
+    int big;         // rows of the large kernel's tile, 256 or 192; 0: not that kernel
+    int bm;          // rows of the tile kernel's tile; 0: the kernel for at most 16 rows
+    int splits;      // slices of K; 1: none
+    int kt_per_split;
+    size_t slabs;    // bytes of fp32 slabs
 };
 
 // Large products: at least this many 256 x 256 tiles run on the 256 x 256 kernel.
@@ -671,25 +816,64 @@ constexpr int64_t kCus = 256;
 
 Fp8Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
     Fp8Plan p{};
+    p.splits = 1;
     const int64_t across = ceil_div(N, gated ? 128 : 256);
     if (M > 128 && ceil_div(M, 256) * across >= kBigTiles) {
         // One workgroup a CU: a launch takes as many rounds as its tiles need.  A 192-row tile takes 5/6 of the time of a
         // 256-row one (1000 x 10001 x 4000 fp32: 104 us in one round of 240 tiles, 123 us in one of 160).
         const int64_t r256 = ceil_div(ceil_div(M, 256) * across, kCus), r192 = ceil_div(ceil_div(M, 192) * across, kCus);
         p.big = 6 * r256 <= 5 * r192 ? 256 : 192;
+        return p;
     }
-    if (gated && !p.big) p.slabs = static_cast<size_t>(2 * 4 * M * N);
+    const int64_t nt = ceil_div(K, kTileK);
+    int64_t groups, want;
+    if (M <= 16) {
+        groups = ceil_div(N, 16);
+        want = 256;
+    } else {
+        p.bm = M <= 32 ? 32 : M <= 128 ? 64 : 128;
+        groups = ceil_div(M, p.bm) * ceil_div(N, p.bm == 128 ? 128 : 64) * (gated ? 2 : 1);
+        want = p.bm == 128 ? 512 : 768;
+    }
+    // Split K where the tiles alone leave CUs idle, into slices of at least eight K-tiles.
+    int64_t splits = groups < want * 3 / 4 ? want / groups : 1;
+    if (splits > nt / 8) splits = nt / 8;
+    if (splits < 1) splits = 1;
+    if (splits > 32) splits = 32;
+    if (splits > 1) {
+        p.kt_per_split = static_cast<int>(ceil_div(nt, splits));
+        p.splits = static_cast<int>(ceil_div(nt, p.kt_per_split));
+    }
+    if (gated && p.bm == 0 && p.splits == 1) p.slabs = static_cast<size_t>(4 * M * N);   // act(g) * u
+    else if (gated) p.slabs = static_cast<size_t>(2 * 4 * M * N) * p.splits;
+    else if (p.splits > 1) p.slabs = static_cast<size_t>(4 * M * N) * p.splits;
+    if (gated && p.splits == 1 && p.bm != 0) p.kt_per_split = static_cast<int>(nt > 0 ? nt : 1);   // one slab a weight
     return p;
 }
 
-template <int OUT>
-int launch_tiles(Fp8Args g, int products, hipStream_t st) {
-    constexpr int BM = 64, BN = 64, kLds = 2 * (BM + BN) * kTileK;
+template <int BM, int BN, int WAVES_M, int WAVES_N, int STAGES, int OUT, bool NATIVE>
+int launch_tile(Fp8Args g, int splits, int products, hipStream_t st) {
+    constexpr int kLds = STAGES * tile_stage_bytes(BM, BN, WAVES_M * WAVES_N);
     g.tiles_m = static_cast<int>(ceil_div(g.M, BM));
     g.tiles_n = static_cast<int>(ceil_div(g.N, BN));
-    const dim3 grid(static_cast<unsigned>(g.tiles_m) * g.tiles_n, 1, products);
-    gemm_fp8_tile_kernel<BM, BN, 2, 2, OUT><<<grid, 256, kLds, st>>>(g);
+    const dim3 grid(static_cast<unsigned>(g.tiles_m) * g.tiles_n, splits, products);
+    if (int rc = allow_lds(reinterpret_cast<const void*>(&gemm_fp8_tile_kernel<BM, BN, WAVES_M, WAVES_N, STAGES, OUT, NATIVE>), kLds)) return rc;
+    gemm_fp8_tile_kernel<BM, BN, WAVES_M, WAVES_N, STAGES, OUT, NATIVE><<<grid, 64 * WAVES_M * WAVES_N, kLds, st>>>(g);
     return check_launch("gemm_fp8_tile_kernel");
+}
+// NATIVE16: the products of a 16-bit output (the slabs' sums included) may use the 8-bit instruction.
+template <int OUT, bool NATIVE16>
+int launch_tiles(const Fp8Plan& p, const Fp8Args& g, int products, hipStream_t st) {
+    if (p.bm == 32) return launch_tile<32, 64, 2, 2, 4, OUT, false>(g, p.splits, products, st);
+    if (p.bm == 64) return launch_tile<64, 64, 2, 2, 4, OUT, false>(g, p.splits, products, st);
+    return launch_tile<128, 128, 2, 2, 2, OUT, NATIVE16>(g, p.splits, products, st);
+}
+
+template <int GROUPS, int OUT, int ACT>
+int launch_rows16(const Fp8Plan& p, const Fp8Args& g, hipStream_t st) {
+    const dim3 grid(static_cast<unsigned>(ceil_div(g.N, ACT != kNoAct ? 16 : GROUPS * 16)), p.splits);
+    gemm_fp8_rows16_kernel<GROUPS, 4, OUT, ACT><<<grid, 512, 0, st>>>(g);
+    return check_launch("gemm_fp8_rows16_kernel");
 }
 
 template <int OUT, int ACT, bool NATIVE, int RF>
@@ -738,9 +922,44 @@ Fp8Args make_args(const uint8_t* x, const float* xs, const uint8_t* w, const flo
 }
 
 template <int OUT>
-int run_product(const Fp8Args& g, const Fp8Plan& plan, hipStream_t st) {
-    if (plan.big) return launch_big<OUT, kNoAct, OUT != MIQ_F32>(plan, g, {}, st);
-    return launch_tiles<OUT>(g, 1, st);
+int run_product(Fp8Args g, const Fp8Plan& p, void* slabs, hipStream_t st) {
+    if (p.big) return launch_big<OUT, kNoAct, OUT != MIQ_F32>(p, g, {}, st);
+    if (p.splits == 1) {
+        if (p.bm == 0) return launch_rows16<1, OUT, kNoAct>(p, g, st);
+        return launch_tiles<OUT, OUT != MIQ_F32>(p, g, 1, st);
+    }
+    void* const out = g.out;
+    g.out = slabs;
+    g.kt_per_split = p.kt_per_split;
+    const int rc = p.bm == 0 ? launch_rows16<1, MIQ_F32, kNoAct>(p, g, st) : launch_tiles<MIQ_F32, OUT != MIQ_F32>(p, g, 1, st);
+    if (rc) return rc;
+    const int64_t groups = ceil_div(g.M * g.N, 256);
+    splitk_sum_kernel<OUT><<<static_cast<unsigned>(groups < 4096 ? groups : 4096), 256, 0, st>>>(static_cast<const float*>(slabs), p.splits,
+                                                                                                g.M, g.N, g.bias, out);
+    return check_launch("splitk_sum_kernel");
+}
+
+template <int ACT>
+int run_gated(Fp8Args g, const Fp8Plan& p, float* slabs, uint8_t* q, float* scale, hipStream_t st) {
+    if (p.big) return launch_big<MIQ_F32, ACT, false>(p, g, {q, scale}, st);
+    g.out = slabs;
+    g.kt_per_split = p.kt_per_split;
+    if (p.bm == 0 && p.splits == 1) {
+        if (int rc = launch_rows16<2, MIQ_F32, ACT>(p, g, st)) return rc;
+        return miq_quantize_blocks_fp8(slabs, MIQ_F32, g.M, g.N, q, scale, st);
+    }
+    if (p.bm == 0) {   // both weights' slabs, one launch each
+        if (int rc = launch_rows16<1, MIQ_F32, kNoAct>(p, g, st)) return rc;
+        g.w[0] = g.w[1];
+        g.ws[0] = g.ws[1];
+        g.out = slabs + static_cast<int64_t>(p.splits) * g.M * g.N;
+        if (int rc = launch_rows16<1, MIQ_F32, kNoAct>(p, g, st)) return rc;
+    } else if (int rc = launch_tiles<MIQ_F32, false>(p, g, 2, st)) {
+        return rc;
+    }
+    const int nblocks = static_cast<int>(ceil_div(g.N, 128));
+    gated_join_kernel<ACT><<<static_cast<unsigned>(ceil_div(g.M * nblocks, 16)), 256, 0, st>>>(slabs, p.splits, g.M, g.N, nblocks, q, scale);
+    return check_launch("gated_join_kernel");
 }
 
 }  // namespace
@@ -767,9 +986,9 @@ extern "C" int miq_gemm_fp8(const uint8_t* x, const float* x_scale, const uint8_
     g.bias = bias;
     g.out = out;
     const Fp8Plan plan = make_plan(M, N, K, false);
-    if (out_dtype == MIQ_F32) return run_product<MIQ_F32>(g, plan, st);
-    if (out_dtype == MIQ_F16) return run_product<MIQ_F16>(g, plan, st);
-    return run_product<MIQ_BF16>(g, plan, st);
+    if (out_dtype == MIQ_F32) return run_product<MIQ_F32>(g, plan, at, st);
+    if (out_dtype == MIQ_F16) return run_product<MIQ_F16>(g, plan, at, st);
+    return run_product<MIQ_BF16>(g, plan, at, st);
 }
 
 extern "C" size_t miq_gated_fp8_workspace(int64_t M, int64_t N, int64_t K) {
@@ -793,17 +1012,7 @@ extern "C" int miq_gated_fp8(const uint8_t* x, const float* x_scale, const uint8
     char* at = static_cast<char*>(workspace);
     Fp8Args g = make_args(x, x_scale, w_gate, gate_scale, w_up, up_scale, M, N, K, at, st);
     const Fp8Plan plan = make_plan(M, N, K, true);
-    if (plan.big)
-        return act == MIQ_ACT_SILU ? launch_big<MIQ_F32, MIQ_ACT_SILU, false>(plan, g, {q, scale}, st)
-                                   : launch_big<MIQ_F32, MIQ_ACT_GELU, false>(plan, g, {q, scale}, st);
-    const int nblocks = static_cast<int>(ceil_div(N, 128));
-    MIQ_REQUIRE(ceil_div(M * nblocks, 16) < (1ll << 24), MIQ_ERANGE, "miq_gated_fp8: too many blocks");
-    g.out = at;
-    g.kt_per_split = g.kblocks > 0 ? g.kblocks : 1;
-    if (int rc = launch_tiles<MIQ_F32>(g, 2, st)) return rc;
-    const unsigned join = static_cast<unsigned>(ceil_div(M * nblocks, 16));
-    const float* slabs = reinterpret_cast<const float*>(at);
-    if (act == MIQ_ACT_SILU) gated_join_kernel<MIQ_ACT_SILU><<<join, 256, 0, st>>>(slabs, 1, M, g.N, nblocks, q, scale);
-    else gated_join_kernel<MIQ_ACT_GELU><<<join, 256, 0, st>>>(slabs, 1, M, g.N, nblocks, q, scale);
-    return check_launch("gated_join_kernel");
+    float* slabs = reinterpret_cast<float*>(at);
+    return act == MIQ_ACT_SILU ? run_gated<MIQ_ACT_SILU>(g, plan, slabs, q, scale, st)
+                               : run_gated<MIQ_ACT_GELU>(g, plan, slabs, q, scale, st);
 }
