@@ -299,29 +299,17 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
     }
 }
 
-// out = the slabs' sum (in order) + bias
-template <int OUT>
-__global__ __launch_bounds__(256) void splitk_sum_kernel(const float* __restrict__ slabs, int splits, int64_t M, int N,
-                                                         const float* __restrict__ bias, void* __restrict__ out) {
-    const int64_t total = M * N;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-        float v = 0.f;
-        for (int s = 0; s < splits; ++s) v += slabs[s * total + i];
-        store_value<OUT>(out, i, bias ? v + bias[i % N] : v);
-    }
-}
-
 // ---- at most 16 rows: the weight streams once, HBM -> registers ------------------------------------------------------
 // A row group of 16 weight rows is one operand fragment, and nothing is shared between waves, so nothing is staged: a lane
-// loads the chunks that the instructions want from it.  A workgroup of eight waves owns GROUPS row groups; wave v sums the
-// K-tiles v, v + 8, ... (eight consecutive K-tiles are 1 KiB of a row), DEPTH of them in flight, and the eight partial sums
-// meet in LDS.  A gated product's groups are the gate's and the up projection's same 16 columns: the workgroup finishes
-// act(g) * u in fp32, and the quantizer follows.
-template <int GROUPS, int DEPTH, int OUT, int ACT>
-__global__ __launch_bounds__(512) void gemm_fp8_rows16_kernel(Fp8Args g) {
+// loads the chunks that the instructions want from it.  A workgroup of kWaves waves owns GROUPS row groups; wave v sums
+// the K-tiles v, v + kWaves, ... (eight consecutive K-tiles are 1 KiB of a row), DEPTH of them in flight, and the partial
+// sums meet in LDS.  A gated product's groups are the gate's and the up projection's of the same columns: the workgroup
+// finishes act(g) * u in fp32, and the quantizer follows.
+template <int GROUPS, int kWaves, int DEPTH, int OUT, int ACT>
+__global__ __launch_bounds__(64 * kWaves) void gemm_fp8_rows16_kernel(Fp8Args g) {
     constexpr bool GATED = ACT != kNoAct;
-    static_assert(!GATED || GROUPS == 2, "a gate's group and an up projection's");
-    constexpr int kWaves = 8, kCols = GATED ? 16 : GROUPS * 16;
+    static_assert(!GATED || GROUPS % 2 == 0, "as many of the gate's groups as of the up projection's");
+    constexpr int kEach = GATED ? GROUPS / 2 : GROUPS, kCols = kEach * 16;   // groups of one weight
     __shared__ float part[kWaves * GROUPS * 256];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -337,8 +325,8 @@ __global__ __launch_bounds__(512) void gemm_fp8_rows16_kernel(Fp8Args g) {
     __amdgpu_buffer_rsrc_t rw[GROUPS];
 #pragma unroll
     for (int j = 0; j < GROUPS; ++j) {
-        const int first = GATED ? 0 : j * 16, left = nrows - first;
-        rw[j] = make_rsrc(g.w[GATED ? j : 0] + static_cast<int64_t>(n0 + first) * g.K,
+        const int first = j % kEach * 16, left = nrows - first;
+        rw[j] = make_rsrc(g.w[j / kEach] + static_cast<int64_t>(n0 + first) * g.K,
                           left > 0 ? static_cast<uint32_t>(left) * static_cast<uint32_t>(g.K) : 0);
     }
     using scalar_floats = const __attribute__((address_space(4))) float*;
@@ -375,7 +363,7 @@ __global__ __launch_bounds__(512) void gemm_fp8_rows16_kernel(Fp8Args g) {
             const int t = kt + u * kWaves, ts = t < kt1 ? t : kt0;   // (a K-tile past the slice: zeros, times some scale)
             const Widened x = widen(ring[u].x);
 #pragma unroll
-            for (int j = 0; j < GROUPS; ++j) add_scaled(acc[j], block_sum(widen(ring[u].w[j]), x), ring[u].s * wscale[GATED ? j : 0][ts]);
+            for (int j = 0; j < GROUPS; ++j) add_scaled(acc[j], block_sum(widen(ring[u].w[j]), x), ring[u].s * wscale[j / kEach][ts]);
             fill(ring[u], t + DEPTH * kWaves);
         }
     }
@@ -391,17 +379,22 @@ __global__ __launch_bounds__(512) void gemm_fp8_rows16_kernel(Fp8Args g) {
         for (int w = 0; w < kWaves; ++w) v += part[w * GROUPS * 256 + at];
         return v;
     };
-    const int e = threadIdx.x;
-    if (e >= 16 * kCols) return;
-    const int m = e / kCols, ch = e % kCols, n = n0 + ch;
-    if (m >= g.M || n >= g.N) return;
     void* out = g.out;
     if (g.kt_per_split) out = static_cast<float*>(out) + static_cast<int64_t>(blockIdx.y) * g.M * g.N;
-    float v;
-    if constexpr (GATED) v = gate_value<ACT>(sum_of(0, m, ch)) * sum_of(1, m, ch);
-    else v = sum_of(ch >> 4, m, ch & 15) + (g.bias && !g.kt_per_split ? g.bias[n] : 0.f);
-    store_value<OUT>(out, static_cast<int64_t>(m) * g.N + n, v);
+    for (int e = threadIdx.x; e < 16 * kCols; e += 64 * kWaves) {
+        const int m = e / kCols, ch = e % kCols, n = n0 + ch;
+        if (m >= g.M || n >= g.N) continue;
+        float v;
+        if constexpr (GATED) v = gate_value<ACT>(sum_of(ch >> 4, m, ch & 15)) * sum_of(kEach + (ch >> 4), m, ch & 15);
+        else v = sum_of(ch >> 4, m, ch & 15) + (g.bias && !g.kt_per_split ? g.bias[n] : 0.f);
+        store_value<OUT>(out, static_cast<int64_t>(m) * g.N + n, v);
+    }
 }
+
+struct GatedOut {
+    uint8_t* q;      // [M, N]
+    float* scale;    // [ceil(N / 128), M]
+};
 
 // ---- 256 x 256 outputs a workgroup: large products -----------------------------------------------------------------
 // Eight waves, 2 (rows) x 4 (columns), a wave owns 128 x 64 outputs: eight row fragments by four column fragments.
@@ -422,10 +415,6 @@ __global__ __launch_bounds__(512) void gemm_fp8_rows16_kernel(Fp8Args g) {
 //
 // GATED: the tile is 128 columns of both weights, a wave's column fragments 0, 1 the gate's and 2, 3 the up projection's
 // same 32 columns, so that a lane holds both factors of its outputs and the 128 columns are one block of the result.
-struct GatedOut {
-    uint8_t* q;      // [M, N]
-    float* scale;    // [ceil(N / 128), M]
-};
 
 template <int OUT, int ACT, bool NATIVE, int RF>
 __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut go) {
@@ -575,7 +564,7 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
 #pragma unroll
             for (int j = 0; j < 4; ++j) wf[j] = operand<NATIVE>(read(wt, w_row(j)));
             rows_step(integral_constant<int, 0>{}, xt, sv0, sw0, sw1);
-            rows_step(integral_constant<int, 1>{}, xt, sv0, sw0, sw1);
+            if constexpr (AS > 1) rows_step(integral_constant<int, 1>{}, xt, sv0, sw0, sw1);
             if constexpr (AS > 2) rows_step(integral_constant<int, 2>{}, xt, sv0, sw0, sw1);
             if constexpr (AS > 3) rows_step(integral_constant<int, 3>{}, xt, sv0, sw0, sw1);
             if (group) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");   // x(t + 1), w(t + 1); x(t + 2) stays in flight
@@ -585,10 +574,13 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
             const int tn1 = t + 1 < nt ? t + 1 : t;
             sv0 = row_scales(tn1, 0);
             const uint32_t sv1_next = row_scales(tn1, 1);
-            if constexpr (AS < 3) rows_step(integral_constant<int, 2>{}, xt, sv1, sw0, sw1);
-            if constexpr (AS < 4) rows_step(integral_constant<int, 3>{}, xt, sv1, sw0, sw1);
-            rows_step(integral_constant<int, 4>{}, xt, sv1, sw0, sw1);
-            rows_step(integral_constant<int, 5>{}, xt, sv1, sw0, sw1);
+            if constexpr (RF == 2) rows_step(integral_constant<int, 1>{}, xt, sv1, sw0, sw1);
+            if constexpr (RF == 4) rows_step(integral_constant<int, 2>{}, xt, sv1, sw0, sw1);
+            if constexpr (RF == 4 || RF == 6) rows_step(integral_constant<int, 3>{}, xt, sv1, sw0, sw1);
+            if constexpr (RF >= 6) {
+                rows_step(integral_constant<int, 4>{}, xt, sv1, sw0, sw1);
+                rows_step(integral_constant<int, 5>{}, xt, sv1, sw0, sw1);
+            }
             if constexpr (RF == 8) {
                 rows_step(integral_constant<int, 6>{}, xt, sv1, sw0, sw1);
                 rows_step(integral_constant<int, 7>{}, xt, sv1, sw0, sw1);
@@ -744,9 +736,56 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
     }
 }
 
-// ---- the gated product's second half -------------------------------------------------------------------------------
+// ---- split products: the slabs' sums ---------------------------------------------------------------------------------
+// Eight consecutive sums of a row, over `splits` slabs in order, `inside` of them in the row.
+template <bool VEC>
+__device__ __forceinline__ void sum_slabs(const float* __restrict__ slabs, int splits, int64_t size, int64_t at, int inside, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    if (VEC ? inside == 8 : false) {
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) {
+            const v4f* p = reinterpret_cast<const v4f*>(slabs + s * size + at);
+            const v4f a = p[0], b = p[1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] += a[i];
+                v[4 + i] += b[i];
+            }
+        }
+        return;
+    }
+#pragma unroll 2
+    for (int s = 0; s < splits; ++s) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < inside) v[i] += slabs[s * size + at + i];
+    }
+}
+
+// out = the slabs' sum + bias; eight columns a thread
+template <int OUT, bool VEC>
+__global__ __launch_bounds__(256) void splitk_sum_kernel(const float* __restrict__ slabs, int splits, int64_t M, int N,
+                                                         const float* __restrict__ bias, void* __restrict__ out) {
+    const int per_row = (N + 7) / 8;
+    const int64_t total = M * per_row;
+    for (int64_t id = blockIdx.x * 256ll + threadIdx.x; id < total; id += gridDim.x * 256ll) {
+        const int64_t m = id / per_row;
+        const int n = static_cast<int>(id % per_row) * 8, inside = N - n < 8 ? N - n : 8;
+        float v[8];
+        sum_slabs<VEC>(slabs, splits, M * N, m * N + n, inside, v);
+        if (bias) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < inside) v[i] += bias[n + i];
+        }
+        store4<OUT>(out, m * N + n, inside, VEC, v4f{v[0], v[1], v[2], v[3]});
+        if (inside > 4) store4<OUT>(out, m * N + n + 4, inside - 4, VEC, v4f{v[4], v[5], v[6], v[7]});
+    }
+}
+
 // h = act(sum of the gate's slabs) * (sum of the up projection's), in blocks: sixteen lanes a block of one row.
-template <int ACT>
+template <int ACT, bool VEC>
 __global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict__ slabs, int splits, int64_t M, int N, int nblocks,
                                                          uint8_t* __restrict__ q, float* __restrict__ scale) {
     const int lane = threadIdx.x & 15;
@@ -755,21 +794,14 @@ __global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict
     const int b = static_cast<int>(id % nblocks), n = b * 128 + lane * 8;
     const int inside = m < M && n < N ? (N - n < 8 ? N - n : 8) : 0;
     const int64_t size = M * N;
-    float h[8];
+    float gate[8], h[8];
+    sum_slabs<VEC>(slabs, splits, size, m * N + n, inside, gate);
+    sum_slabs<VEC>(slabs + splits * size, splits, size, m * N + n, inside, h);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        h[i] = 0.0f;
-        if (i < inside) {
-            const int64_t o = m * N + n + i;
-            float gate = 0.0f, up = 0.0f;
-            for (int s = 0; s < splits; ++s) gate += slabs[s * size + o];
-            for (int s = 0; s < splits; ++s) up += slabs[(splits + s) * size + o];
-            h[i] = gate_value<ACT>(gate) * up;
-        }
-    }
+    for (int i = 0; i < 8; ++i) h[i] = gate_value<ACT>(gate[i]) * h[i];   // (0 past the row)
     uint32_t c[2];
     const float s = quantize8_in_row(h, c);
-    store8_codes<false>(q, m * N + n, inside, c);
+    store8_codes<VEC>(q, m * N + n, inside, c);
     if (lane == 0 && m < M) scale[static_cast<int64_t>(b) * M + m] = s;
 }
 
@@ -818,6 +850,9 @@ Fp8Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
     Fp8Plan p{};
     p.splits = 1;
     const int64_t across = ceil_div(N, gated ? 128 : 256);
+#ifdef FORCE_BIG
+    p.big = FORCE_BIG; return p;
+#endif
     if (M > 128 && ceil_div(M, 256) * across >= kBigTiles) {
         // One workgroup a CU: a launch takes as many rounds as its tiles need.  A 192-row tile takes 5/6 of the time of a
         // 256-row one (1000 x 10001 x 4000 fp32: 104 us in one round of 240 tiles, 123 us in one of 160).
@@ -864,16 +899,25 @@ int launch_tile(Fp8Args g, int splits, int products, hipStream_t st) {
 // NATIVE16: the products of a 16-bit output (the slabs' sums included) may use the 8-bit instruction.
 template <int OUT, bool NATIVE16>
 int launch_tiles(const Fp8Plan& p, const Fp8Args& g, int products, hipStream_t st) {
-    if (p.bm == 32) return launch_tile<32, 64, 2, 2, 4, OUT, false>(g, p.splits, products, st);
-    if (p.bm == 64) return launch_tile<64, 64, 2, 2, 4, OUT, false>(g, p.splits, products, st);
+    if (p.bm == 32) return launch_tile<32, 64, 2, 2, 4, OUT, NATIVE16>(g, p.splits, products, st);
+    if (p.bm == 64) return launch_tile<64, 64, 2, 2, 4, OUT, NATIVE16>(g, p.splits, products, st);
     return launch_tile<128, 128, 2, 2, 2, OUT, NATIVE16>(g, p.splits, products, st);
 }
 
 template <int GROUPS, int OUT, int ACT>
 int launch_rows16(const Fp8Plan& p, const Fp8Args& g, hipStream_t st) {
-    const dim3 grid(static_cast<unsigned>(ceil_div(g.N, ACT != kNoAct ? 16 : GROUPS * 16)), p.splits);
-    gemm_fp8_rows16_kernel<GROUPS, 4, OUT, ACT><<<grid, 512, 0, st>>>(g);
+    // Two K-tiles in flight a wave: with four a wave holds 100 registers instead of 58 and fewer fit a SIMD (1 x 4096 x 14336:
+    // 11.7 us against 12.6; 1 x 28672 x 8192 44.3 against 47.6).
+    const dim3 grid(static_cast<unsigned>(ceil_div(g.N, ACT != kNoAct ? GROUPS * 8 : GROUPS * 16)), p.splits);
+    gemm_fp8_rows16_kernel<GROUPS, 8, 2, OUT, ACT><<<grid, 512, 0, st>>>(g);
     return check_launch("gemm_fp8_rows16_kernel");
+}
+template <int OUT>
+int launch_rows16_linear(const Fp8Plan& p, const Fp8Args& g, hipStream_t st) {
+    // 32 columns a workgroup where a wave has few K-tiles to stream and that still gives every CU a workgroup (1 x 14336 x 4096:
+    // 14.1 us against 15.8 with 16 columns), 16 elsewhere (1 x 4096 x 14336: 11.7 against 17.4, 1 x 28672 x 8192: 44 against 56).
+    if (p.splits == 1 && g.kblocks <= 48 && ceil_div(g.N, 32) >= kCus) return launch_rows16<2, OUT, kNoAct>(p, g, st);
+    return launch_rows16<1, OUT, kNoAct>(p, g, st);
 }
 
 template <int OUT, int ACT, bool NATIVE, int RF>
@@ -888,7 +932,10 @@ int launch_big_rows(Fp8Args g, GatedOut go, hipStream_t st) {
 }
 template <int OUT, int ACT, bool NATIVE>
 int launch_big(const Fp8Plan& plan, const Fp8Args& g, GatedOut go, hipStream_t st) {
-    return plan.big == 256 ? launch_big_rows<OUT, ACT, NATIVE, 8>(g, go, st) : launch_big_rows<OUT, ACT, NATIVE, 6>(g, go, st);
+    if (plan.big == 256) return launch_big_rows<OUT, ACT, NATIVE, 8>(g, go, st);
+    if (plan.big == 192) return launch_big_rows<OUT, ACT, NATIVE, 6>(g, go, st);
+    if (plan.big == 128) return launch_big_rows<OUT, ACT, NATIVE, 4>(g, go, st);
+    return launch_big_rows<OUT, ACT, NATIVE, 2>(g, go, st);
 }
 
 // Checks that both products share; `weights` of them, 1 or 2.
@@ -925,7 +972,7 @@ template <int OUT>
 int run_product(Fp8Args g, const Fp8Plan& p, void* slabs, hipStream_t st) {
     if (p.big) return launch_big<OUT, kNoAct, OUT != MIQ_F32>(p, g, {}, st);
     if (p.splits == 1) {
-        if (p.bm == 0) return launch_rows16<1, OUT, kNoAct>(p, g, st);
+        if (p.bm == 0) return launch_rows16_linear<OUT>(p, g, st);
         return launch_tiles<OUT, OUT != MIQ_F32>(p, g, 1, st);
     }
     void* const out = g.out;
@@ -933,9 +980,11 @@ int run_product(Fp8Args g, const Fp8Plan& p, void* slabs, hipStream_t st) {
     g.kt_per_split = p.kt_per_split;
     const int rc = p.bm == 0 ? launch_rows16<1, MIQ_F32, kNoAct>(p, g, st) : launch_tiles<MIQ_F32, OUT != MIQ_F32>(p, g, 1, st);
     if (rc) return rc;
-    const int64_t groups = ceil_div(g.M * g.N, 256);
-    splitk_sum_kernel<OUT><<<static_cast<unsigned>(groups < 4096 ? groups : 4096), 256, 0, st>>>(static_cast<const float*>(slabs), p.splits,
-                                                                                                g.M, g.N, g.bias, out);
+    const int64_t groups = ceil_div(g.M * ceil_div(g.N, 8), 256);
+    const unsigned grid = static_cast<unsigned>(groups < 8192 ? groups : 8192);
+    const float* sums = static_cast<const float*>(slabs);
+    if (g.N % 8 == 0) splitk_sum_kernel<OUT, true><<<grid, 256, 0, st>>>(sums, p.splits, g.M, g.N, g.bias, out);
+    else splitk_sum_kernel<OUT, false><<<grid, 256, 0, st>>>(sums, p.splits, g.M, g.N, g.bias, out);
     return check_launch("splitk_sum_kernel");
 }
 
@@ -958,7 +1007,9 @@ int run_gated(Fp8Args g, const Fp8Plan& p, float* slabs, uint8_t* q, float* scal
         return rc;
     }
     const int nblocks = static_cast<int>(ceil_div(g.N, 128));
-    gated_join_kernel<ACT><<<static_cast<unsigned>(ceil_div(g.M * nblocks, 16)), 256, 0, st>>>(slabs, p.splits, g.M, g.N, nblocks, q, scale);
+    const unsigned grid = static_cast<unsigned>(ceil_div(g.M * nblocks, 16));
+    if (g.N % 8 == 0) gated_join_kernel<ACT, true><<<grid, 256, 0, st>>>(slabs, p.splits, g.M, g.N, nblocks, q, scale);
+    else gated_join_kernel<ACT, false><<<grid, 256, 0, st>>>(slabs, p.splits, g.M, g.N, nblocks, q, scale);
     return check_launch("gated_join_kernel");
 }
 
