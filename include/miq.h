@@ -425,7 +425,7 @@ int miq_rms_norm_fp8(const void* x, const void* residual, const void* weight, in
  * The product of two scales has to be a finite fp32 number.
  * M, N below 2^31, K below 2^22, at most 2^22 tiles of 64 x 64 outputs (MIQ_ERANGE otherwise).
  * workspace: at least miq_gemm_fp8_workspace(...) bytes, 256-byte aligned; may be NULL when that is 0. */
-size_t miq_gemm_fp8_workspace(int64_t M, int64_t N, int64_t K);
+size_t miq_gemm_fp8_workspace(int64_t M, int64_t N, int64_t K, int out_dtype);
 int miq_gemm_fp8(const uint8_t* x, const float* x_scale, const uint8_t* w, const float* w_scale, int64_t M, int64_t N, int64_t K,
                  const float* bias, void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
 

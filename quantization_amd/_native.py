@@ -74,7 +74,7 @@ SYMBOLS = {
     "miq_quantize_blocks_fp8": (_int, [_p, _int, _i64, _i64, _p, _p, _p]),
     "miq_quantize_weight_fp8": (_int, [_p, _int, _i64, _i64, _p, _p, _p]),
     "miq_rms_norm_fp8": (_int, [_p, _p, _p, _int, _int, _i64, _i64, ctypes.c_float, _p, _p, _p, _p]),
-    "miq_gemm_fp8_workspace": (_size, [_i64] * 3),
+    "miq_gemm_fp8_workspace": (_size, [_i64] * 3 + [_int]),
     "miq_gemm_fp8": (_int, [_p] * 4 + [_i64] * 3 + [_p, _p, _int, _p, _size, _p]),
     "miq_gated_fp8_workspace": (_size, [_i64] * 3),
     "miq_gated_fp8": (_int, [_p] * 6 + [_i64] * 3 + [_int, _p, _p, _p, _size, _p]),
@@ -905,7 +905,7 @@ def gemm_fp8(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16):
     bias = _f32_vec(bias, N, "bias", x.device)
     out = x.new_empty((M, N), dtype=out_dtype)
     L = lib()
-    need = L.miq_gemm_fp8_workspace(M, N, K)
+    need = L.miq_gemm_fp8_workspace(M, N, K, code)
     ws = x.new_empty(need, dtype=torch.uint8) if need else None
     _launch(L.miq_gemm_fp8, index, x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), M, N, K,
             None if bias is None else bias.data_ptr(), out.data_ptr(), code, None if ws is None else ws.data_ptr(), need)

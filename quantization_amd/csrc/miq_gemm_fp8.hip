@@ -28,9 +28,10 @@ struct Fp8Args {
     const float* bias;     // [N] or null
     void* out;             // [M, N]; slabs [splits][M][N] (for each weight) of a split product
     int64_t M;
-    int N, K, kblocks;
+    int N, K, kblocks;     // K: bytes between two rows of x and w, a multiple of 16
     int tiles_m, tiles_n;
     int kt_per_split;      // K-tiles each blockIdx.y slice sums; 0 = all, straight to `out`
+    int pitch;             // floats between two rows of a slab: N rounded up to 8 (columns past N hold zeros)
 };
 
 // A fragment of 16 rows and one K-tile: the lane's 16-byte chunks (lane >> 4) and 4 + (lane >> 4) of row lane & 15.
@@ -147,21 +148,30 @@ __device__ __forceinline__ void stage_rows(const uint8_t* rows, int nrows, int K
     }
 }
 
-// Rows of K bytes -> rows of `pitch` bytes (K rounded up to 16), zeros past K: one thread a 16-byte piece.
-__global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* __restrict__ src, int64_t rows, int K, int pitch,
-                                                       uint8_t* __restrict__ dst) {
-    const int per_row = pitch / kChunk;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * per_row; i += gridDim.x * 256ll) {
-        const int64_t r = i / per_row;
-        const int k = static_cast<int>(i % per_row) * kChunk;
-        const uint8_t* p = src + r * K + k;
-        v4i v = {0, 0, 0, 0};
-        if (K - k >= kChunk) {
-            __builtin_memcpy(&v, p, kChunk);
-        } else {
-            for (int b = 0; b < K - k; ++b) v[b >> 2] |= static_cast<int>(static_cast<uint32_t>(p[b]) << (8 * (b & 3)));
+// Rows of K bytes -> rows of `pitch` bytes (K rounded up to 16), zeros past K: one thread a 16-byte piece, up to three
+// matrices in one launch.
+struct PadArgs {
+    const uint8_t* src[3];
+    uint8_t* dst[3];
+    int64_t rows[3];   // 0: none
+    int K, pitch;
+};
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs a) {
+    const int per_row = a.pitch / kChunk;
+#pragma unroll
+    for (int o = 0; o < 3; ++o) {
+        for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < a.rows[o] * per_row; i += gridDim.x * 256ll) {
+            const int64_t r = i / per_row;
+            const int k = static_cast<int>(i % per_row) * kChunk;
+            const uint8_t* p = a.src[o] + r * a.K + k;
+            v4i v = {0, 0, 0, 0};
+            if (a.K - k >= kChunk) {
+                __builtin_memcpy(&v, p, kChunk);
+            } else {
+                for (int b = 0; b < a.K - k; ++b) v[b >> 2] |= static_cast<int>(static_cast<uint32_t>(p[b]) << (8 * (b & 3)));
+            }
+            *reinterpret_cast<v4i*>(a.dst[o] + i * kChunk) = v;
         }
-        *reinterpret_cast<v4i*>(dst + i * kChunk) = v;
     }
 }
 
@@ -217,7 +227,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
     const int kt1 = g.kt_per_split && kt0 + g.kt_per_split < g.kblocks ? kt0 + g.kt_per_split : g.kblocks;
     void* out = g.out;
     if constexpr (OUT == MIQ_F32) {
-        if (g.kt_per_split) out = static_cast<float*>(out) + (static_cast<int64_t>(which) * gridDim.y + blockIdx.y) * g.M * g.N;
+        if (g.kt_per_split) out = static_cast<float*>(out) + (static_cast<int64_t>(which) * gridDim.y + blockIdx.y) * g.M * g.pitch;
     }
 
     v4f acc[FM][FN] = {};
@@ -282,11 +292,12 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
     }
 
     // A fragment's results: 4 * (lane >> 4) + register -> column n, lane & 15 -> row m.
-    const bool vec = (g.N & 3) == 0;
+    const int cols = g.kt_per_split ? g.pitch : g.N;   // of a row of `out`
+    const bool vec = (cols & 3) == 0;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
         const int n = n0 + wn * WN + j * 16 + (lane >> 4) * 4;
-        if (n >= g.N) continue;
+        if (n >= cols) continue;
         v4f b = {0.f, 0.f, 0.f, 0.f};
         if (g.bias && !g.kt_per_split)
             for (int e = 0; e < 4; ++e)
@@ -294,7 +305,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             const int64_t m = m0 + wm * WM + i * 16 + (lane & 15);
-            if (m < g.M) store4<OUT>(out, m * g.N + n, g.N - n, vec, acc[i][j] + b);
+            if (m < g.M) store4<OUT>(out, m * cols + n, cols - n, vec, acc[i][j] + b);
         }
     }
 }
@@ -380,14 +391,15 @@ __global__ __launch_bounds__(64 * kWaves) void gemm_fp8_rows16_kernel(Fp8Args g)
         return v;
     };
     void* out = g.out;
-    if (g.kt_per_split) out = static_cast<float*>(out) + static_cast<int64_t>(blockIdx.y) * g.M * g.N;
+    const int cols = g.kt_per_split ? g.pitch : g.N;   // of a row of `out`
+    if (g.kt_per_split) out = static_cast<float*>(out) + static_cast<int64_t>(blockIdx.y) * g.M * cols;
     for (int e = threadIdx.x; e < 16 * kCols; e += 64 * kWaves) {
         const int m = e / kCols, ch = e % kCols, n = n0 + ch;
-        if (m >= g.M || n >= g.N) continue;
+        if (m >= g.M || n >= cols) continue;
         float v;
         if constexpr (GATED) v = gate_value<ACT>(sum_of(ch >> 4, m, ch & 15)) * sum_of(kEach + (ch >> 4), m, ch & 15);
         else v = sum_of(ch >> 4, m, ch & 15) + (g.bias && !g.kt_per_split ? g.bias[n] : 0.f);
-        store_value<OUT>(out, static_cast<int64_t>(m) * g.N + n, v);
+        store_value<OUT>(out, static_cast<int64_t>(m) * cols + n, v);
     }
 }
 
@@ -737,72 +749,65 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
 }
 
 // ---- split products: the slabs' sums ---------------------------------------------------------------------------------
-// Eight consecutive sums of a row, over `splits` slabs in order, `inside` of them in the row.
-template <bool VEC>
-__device__ __forceinline__ void sum_slabs(const float* __restrict__ slabs, int splits, int64_t size, int64_t at, int inside, float (&v)[8]) {
+// Eight consecutive sums of a row at `at`, over `splits` slabs of `size` floats, in order.
+__device__ __forceinline__ void sum_slabs(const float* __restrict__ slabs, int splits, int64_t size, int64_t at, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    if (VEC ? inside == 8 : false) {
 #pragma unroll 4
-        for (int s = 0; s < splits; ++s) {
-            const v4f* p = reinterpret_cast<const v4f*>(slabs + s * size + at);
-            const v4f a = p[0], b = p[1];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] += a[i];
-                v[4 + i] += b[i];
-            }
-        }
-        return;
-    }
-#pragma unroll 2
     for (int s = 0; s < splits; ++s) {
+        const v4f* p = reinterpret_cast<const v4f*>(slabs + s * size + at);
+        const v4f a = p[0], b = p[1];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < inside) v[i] += slabs[s * size + at + i];
+        for (int i = 0; i < 4; ++i) {
+            v[i] += a[i];
+            v[4 + i] += b[i];
+        }
     }
 }
 
-// out = the slabs' sum + bias; eight columns a thread
-template <int OUT, bool VEC>
-__global__ __launch_bounds__(256) void splitk_sum_kernel(const float* __restrict__ slabs, int splits, int64_t M, int N,
-                                                         const float* __restrict__ bias, void* __restrict__ out) {
-    const int per_row = (N + 7) / 8;
-    const int64_t total = M * per_row;
+// out = the slabs' sum + bias; eight columns a thread (slab rows are a multiple of 8 long)
+template <int OUT>
+__global__ __launch_bounds__(256) void splitk_sum_kernel(const float* __restrict__ slabs, int splits, Fp8Args g, void* __restrict__ out) {
+    const int per_row = g.pitch / 8;
+    const int64_t total = g.M * per_row;
+    const bool vec = (g.N & 3) == 0;
     for (int64_t id = blockIdx.x * 256ll + threadIdx.x; id < total; id += gridDim.x * 256ll) {
         const int64_t m = id / per_row;
-        const int n = static_cast<int>(id % per_row) * 8, inside = N - n < 8 ? N - n : 8;
+        const int n = static_cast<int>(id % per_row) * 8;
         float v[8];
-        sum_slabs<VEC>(slabs, splits, M * N, m * N + n, inside, v);
-        if (bias) {
+        sum_slabs(slabs, splits, g.M * g.pitch, m * g.pitch + n, v);
+        if (g.bias) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (i < inside) v[i] += bias[n + i];
+                if (n + i < g.N) v[i] += g.bias[n + i];
         }
-        store4<OUT>(out, m * N + n, inside, VEC, v4f{v[0], v[1], v[2], v[3]});
-        if (inside > 4) store4<OUT>(out, m * N + n + 4, inside - 4, VEC, v4f{v[4], v[5], v[6], v[7]});
+        store4<OUT>(out, m * g.N + n, g.N - n, vec, v4f{v[0], v[1], v[2], v[3]});
+        store4<OUT>(out, m * g.N + n + 4, g.N - n - 4, vec, v4f{v[4], v[5], v[6], v[7]});
     }
 }
 
 // h = act(sum of the gate's slabs) * (sum of the up projection's), in blocks: sixteen lanes a block of one row.
-template <int ACT, bool VEC>
-__global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict__ slabs, int splits, int64_t M, int N, int nblocks,
+template <int ACT>
+__global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict__ slabs, int splits, Fp8Args g, int nblocks,
                                                          uint8_t* __restrict__ q, float* __restrict__ scale) {
     const int lane = threadIdx.x & 15;
     const int64_t id = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
     const int64_t m = id / nblocks;
     const int b = static_cast<int>(id % nblocks), n = b * 128 + lane * 8;
-    const int inside = m < M && n < N ? (N - n < 8 ? N - n : 8) : 0;
-    const int64_t size = M * N;
-    float gate[8], h[8];
-    sum_slabs<VEC>(slabs, splits, size, m * N + n, inside, gate);
-    sum_slabs<VEC>(slabs + splits * size, splits, size, m * N + n, inside, h);
+    const int64_t size = g.M * g.pitch;
+    float gate[8] = {}, h[8] = {};
+    if (m < g.M && n < g.pitch) {
+        sum_slabs(slabs, splits, size, m * g.pitch + n, gate);
+        sum_slabs(slabs + splits * size, splits, size, m * g.pitch + n, h);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) h[i] = gate_value<ACT>(gate[i]) * h[i];   // (0 past the row)
     uint32_t c[2];
     const float s = quantize8_in_row(h, c);
-    store8_codes<VEC>(q, m * N + n, inside, c);
-    if (lane == 0 && m < M) scale[static_cast<int64_t>(b) * M + m] = s;
+    const int inside = m < g.M && n < g.N ? (g.N - n < 8 ? g.N - n : 8) : 0;
+    if ((g.N & 7) == 0) store8_codes<true>(q, m * g.N + n, inside, c);
+    else store8_codes<false>(q, m * g.N + n, inside, c);
+    if (lane == 0 && m < g.M) scale[static_cast<int64_t>(b) * g.M + m] = s;
 }
 
 // Every size that the kernels index with 32 bits, bounded before any arithmetic.
@@ -824,43 +829,61 @@ int64_t pitch_of(int64_t K) { return round_up(K, kChunk); }
 size_t padded_bytes(int64_t M, int64_t N, int64_t weights, int64_t K) {
     return K % kChunk == 0 ? 0 : align256(M * pitch_of(K)) + static_cast<size_t>(weights) * align256(N * pitch_of(K));
 }
-const uint8_t* pad_rows(const uint8_t* src, int64_t rows, int64_t K, char*& at, hipStream_t st) {
-    uint8_t* dst = reinterpret_cast<uint8_t*>(at);
-    const int64_t pieces = rows * (pitch_of(K) / kChunk), groups = ceil_div(pieces, 256);
-    pad_rows_kernel<<<static_cast<unsigned>(groups < 16384 ? groups : 16384), 256, 0, st>>>(src, rows, static_cast<int>(K),
-                                                                                            static_cast<int>(pitch_of(K)), dst);
-    at += align256(rows * pitch_of(K));
-    return dst;
-}
-
 // What a product is cut into: which kernel, how K is split, and how much workspace that needs behind the padded operands.
 struct Fp8Plan {
-    int big;         // rows of the large kernel's tile, 256 or 192; 0: not that kernel
+    int big;         // rows of the large kernel's tile, 256, 192, 128 or 64; 0: not that kernel
     int bm;          // rows of the tile kernel's tile; 0: the kernel for at most 16 rows
     int splits;      // slices of K; 1: none
     int kt_per_split;
     size_t slabs;    // bytes of fp32 slabs
 };
 
-// Large products: at least this many 256 x 256 tiles run on the 256 x 256 kernel.
-constexpr int64_t kBigTiles = 128;
 constexpr int64_t kCus = 256;
 
-Fp8Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
+// Above 16 rows either kernel can run a product; the one with the smaller estimate does.
+//
+// The large kernel has one workgroup a CU: a launch takes as many rounds as its tiles need, and a round a time for each
+// K-tile that hardly depends on the rest.  Measured, us a K-tile and round for tiles of 256, 192, 128, 64 rows: bf16 form
+// (fp32 out, gated) 3.3 2.7 2.15 1.6, 8-bit form 1.8 1.5 1.2 1.0; a few us of prologue and epilogue on top.  The tile kernel
+// fills the chip with small tiles or slices of K and is bound by its own vector and matrix work (128 x 128 tiles 0.75 and
+// 1.0 PFLOP/s, thin tiles 0.55 and 0.9) or by the weight's stream (about 5 TB/s), on top of 8 us of launches.  E.g., us on the
+// tile kernel | the large one: 1024x4096x4096 bf16 37 | 33 (64 rows), 2048x4096x4096 bf16 73 | 41 (128), gated 256x14336x4096
+// 78 | 72 (128), gated 512x4096x4096 46 | 52, 512x4096x4096 bf16 27 | 33, fp32 1024x4096x4096 47 | 51.
+struct BigChoice {
+    int rows;
+    double us;
+};
+BigChoice best_big(int64_t M, int64_t N, int64_t nt, bool gated, bool native) {
+    static constexpr int kTall[4] = {256, 192, 128, 64};
+    static constexpr double kUs[2][4] = {{3.3, 2.7, 2.15, 1.6}, {1.8, 1.5, 1.2, 1.0}};
+    const int64_t across = ceil_div(N, gated ? 128 : 256);
+    BigChoice best{256, 1e30};
+    for (int i = 0; i < 4; ++i) {
+        const double rounds = static_cast<double>(ceil_div(ceil_div(M, kTall[i]) * across, kCus));
+        const double us = rounds * (kUs[native][i] * static_cast<double>(nt) + 4.0);
+        if (us < best.us) best = {kTall[i], us};
+    }
+    best.us += 4.0;
+    return best;
+}
+double tile_us(int64_t M, int64_t N, int64_t K, bool gated, bool native) {
+    const double flops = (gated ? 4.0 : 2.0) * static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
+    const double rate = M > 128 ? (native ? 1.0e9 : 0.75e9) : (native ? 0.9e9 : 0.55e9);   // a us
+    const double work = flops / rate, stream = (gated ? 2.0 : 1.0) * static_cast<double>(N) * static_cast<double>(K) / 5.0e6;
+    return 8.0 + (work > stream ? work : stream);
+}
+
+Fp8Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated, bool native) {
     Fp8Plan p{};
     p.splits = 1;
-    const int64_t across = ceil_div(N, gated ? 128 : 256);
-#ifdef FORCE_BIG
-    p.big = FORCE_BIG; return p;
-#endif
-    if (M > 128 && ceil_div(M, 256) * across >= kBigTiles) {
-        // One workgroup a CU: a launch takes as many rounds as its tiles need.  A 192-row tile takes 5/6 of the time of a
-        // 256-row one (1000 x 10001 x 4000 fp32: 104 us in one round of 240 tiles, 123 us in one of 160).
-        const int64_t r256 = ceil_div(ceil_div(M, 256) * across, kCus), r192 = ceil_div(ceil_div(M, 192) * across, kCus);
-        p.big = 6 * r256 <= 5 * r192 ? 256 : 192;
-        return p;
-    }
     const int64_t nt = ceil_div(K, kTileK);
+    if (M > 16) {
+        const BigChoice big = best_big(M, N, nt, gated, native);
+        if (M > 4096 || big.us <= tile_us(M, N, K, gated, native)) {
+            p.big = big.rows;
+            return p;
+        }
+    }
     int64_t groups, want;
     if (M <= 16) {
         groups = ceil_div(N, 16);
@@ -879,9 +902,10 @@ Fp8Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
         p.kt_per_split = static_cast<int>(ceil_div(nt, splits));
         p.splits = static_cast<int>(ceil_div(nt, p.kt_per_split));
     }
+    const int64_t slab = 4 * M * round_up(N, 8);
     if (gated && p.bm == 0 && p.splits == 1) p.slabs = static_cast<size_t>(4 * M * N);   // act(g) * u
-    else if (gated) p.slabs = static_cast<size_t>(2 * 4 * M * N) * p.splits;
-    else if (p.splits > 1) p.slabs = static_cast<size_t>(4 * M * N) * p.splits;
+    else if (gated) p.slabs = static_cast<size_t>(2 * slab) * p.splits;
+    else if (p.splits > 1) p.slabs = static_cast<size_t>(slab) * p.splits;
     if (gated && p.splits == 1 && p.bm != 0) p.kt_per_split = static_cast<int>(nt > 0 ? nt : 1);   // one slab a weight
     return p;
 }
@@ -938,10 +962,9 @@ int launch_big(const Fp8Plan& plan, const Fp8Args& g, GatedOut go, hipStream_t s
     return launch_big_rows<OUT, ACT, NATIVE, 2>(g, go, st);
 }
 
-// Checks that both products share; `weights` of them, 1 or 2.
-size_t workspace_of(const char* who, int64_t M, int64_t N, int64_t K, bool gated) {
+size_t workspace_of(const char* who, int64_t M, int64_t N, int64_t K, bool gated, bool native) {
     if (check_sizes(who, M, N, K) != MIQ_OK || M == 0 || N == 0) return 0;
-    return padded_bytes(M, N, gated ? 2 : 1, K) + make_plan(M, N, K, gated).slabs;
+    return padded_bytes(M, N, gated ? 2 : 1, K) + make_plan(M, N, K, gated, native).slabs;
 }
 int check_workspace(const char* who, size_t need, const void* workspace, size_t bytes) {
     MIQ_REQUIRE(need == 0 || (workspace && bytes >= need), MIQ_EWORKSPACE, "%s: %zu bytes of workspace needed, %zu given", who, need,
@@ -954,17 +977,29 @@ int check_workspace(const char* who, size_t need, const void* workspace, size_t 
 Fp8Args make_args(const uint8_t* x, const float* xs, const uint8_t* w, const float* ws, const uint8_t* w2, const float* ws2, int64_t M,
                   int64_t N, int64_t K, char*& at, hipStream_t st) {
     Fp8Args g{};
-    const bool pad = K % kChunk != 0;
-    g.x = pad ? pad_rows(x, M, K, at, st) : x;
+    g.x = x;
     g.xs = xs;
-    g.w[0] = pad ? pad_rows(w, N, K, at, st) : w;
-    g.w[1] = pad && w2 ? pad_rows(w2, N, K, at, st) : w2;
+    g.w[0] = w;
+    g.w[1] = w2;
     g.ws[0] = ws;
     g.ws[1] = ws2;
     g.M = M;
     g.N = static_cast<int>(N);
     g.K = static_cast<int>(pitch_of(K));
     g.kblocks = static_cast<int>(ceil_div(K, kTileK));
+    g.pitch = static_cast<int>(round_up(N, 8));
+    if (K % kChunk != 0) {
+        PadArgs a{{x, w, w2}, {}, {M, N, w2 ? N : 0}, static_cast<int>(K), g.K};
+        for (int o = 0; o < 3; ++o) {
+            a.dst[o] = reinterpret_cast<uint8_t*>(at);
+            at += align256(a.rows[o] * g.K);
+        }
+        g.x = a.dst[0];
+        g.w[0] = a.dst[1];
+        if (w2) g.w[1] = a.dst[2];
+        const int64_t groups = ceil_div((M > N ? M : N) * (g.K / kChunk), 256);
+        pad_rows_kernel<<<static_cast<unsigned>(groups < 16384 ? groups : 16384), 256, 0, st>>>(a);
+    }
     return g;
 }
 
@@ -980,11 +1015,9 @@ int run_product(Fp8Args g, const Fp8Plan& p, void* slabs, hipStream_t st) {
     g.kt_per_split = p.kt_per_split;
     const int rc = p.bm == 0 ? launch_rows16<1, MIQ_F32, kNoAct>(p, g, st) : launch_tiles<MIQ_F32, OUT != MIQ_F32>(p, g, 1, st);
     if (rc) return rc;
-    const int64_t groups = ceil_div(g.M * ceil_div(g.N, 8), 256);
-    const unsigned grid = static_cast<unsigned>(groups < 8192 ? groups : 8192);
-    const float* sums = static_cast<const float*>(slabs);
-    if (g.N % 8 == 0) splitk_sum_kernel<OUT, true><<<grid, 256, 0, st>>>(sums, p.splits, g.M, g.N, g.bias, out);
-    else splitk_sum_kernel<OUT, false><<<grid, 256, 0, st>>>(sums, p.splits, g.M, g.N, g.bias, out);
+    const int64_t groups = ceil_div(g.M * (g.pitch / 8), 256);
+    splitk_sum_kernel<OUT><<<static_cast<unsigned>(groups < 8192 ? groups : 8192), 256, 0, st>>>(static_cast<const float*>(slabs), p.splits,
+                                                                                                g, out);
     return check_launch("splitk_sum_kernel");
 }
 
@@ -1001,22 +1034,20 @@ int run_gated(Fp8Args g, const Fp8Plan& p, float* slabs, uint8_t* q, float* scal
         if (int rc = launch_rows16<1, MIQ_F32, kNoAct>(p, g, st)) return rc;
         g.w[0] = g.w[1];
         g.ws[0] = g.ws[1];
-        g.out = slabs + static_cast<int64_t>(p.splits) * g.M * g.N;
+        g.out = slabs + static_cast<int64_t>(p.splits) * g.M * g.pitch;
         if (int rc = launch_rows16<1, MIQ_F32, kNoAct>(p, g, st)) return rc;
     } else if (int rc = launch_tiles<MIQ_F32, false>(p, g, 2, st)) {
         return rc;
     }
     const int nblocks = static_cast<int>(ceil_div(g.N, 128));
-    const unsigned grid = static_cast<unsigned>(ceil_div(g.M * nblocks, 16));
-    if (g.N % 8 == 0) gated_join_kernel<ACT, true><<<grid, 256, 0, st>>>(slabs, p.splits, g.M, g.N, nblocks, q, scale);
-    else gated_join_kernel<ACT, false><<<grid, 256, 0, st>>>(slabs, p.splits, g.M, g.N, nblocks, q, scale);
+    gated_join_kernel<ACT><<<static_cast<unsigned>(ceil_div(g.M * nblocks, 16)), 256, 0, st>>>(slabs, p.splits, g, nblocks, q, scale);
     return check_launch("gated_join_kernel");
 }
 
 }  // namespace
 
-extern "C" size_t miq_gemm_fp8_workspace(int64_t M, int64_t N, int64_t K) {
-    return workspace_of("miq_gemm_fp8_workspace", M, N, K, false);
+extern "C" size_t miq_gemm_fp8_workspace(int64_t M, int64_t N, int64_t K, int out_dtype) {
+    return workspace_of("miq_gemm_fp8_workspace", M, N, K, false, out_dtype != MIQ_F32);
 }
 
 extern "C" int miq_gemm_fp8(const uint8_t* x, const float* x_scale, const uint8_t* w, const float* w_scale, int64_t M, int64_t N,
@@ -1030,20 +1061,20 @@ extern "C" int miq_gemm_fp8(const uint8_t* x, const float* x_scale, const uint8_
     MIQ_REQUIRE(aligned(x_scale, 4) && aligned(w_scale, 4) && aligned(bias, 4) && aligned(out, 16), MIQ_EALIGN,
                 "miq_gemm_fp8: scales and bias must be 4-byte, out 16-byte aligned");
     MIQ_REQUIRE(K % kChunk != 0 || (aligned(x, 16) && aligned(w, 16)), MIQ_EALIGN, "miq_gemm_fp8: x and w must be 16-byte aligned");
-    if (int rc = check_workspace("miq_gemm_fp8", miq_gemm_fp8_workspace(M, N, K), workspace, workspace_bytes)) return rc;
+    if (int rc = check_workspace("miq_gemm_fp8", miq_gemm_fp8_workspace(M, N, K, out_dtype), workspace, workspace_bytes)) return rc;
     const hipStream_t st = as_stream(stream);
     char* at = static_cast<char*>(workspace);
     Fp8Args g = make_args(x, x_scale, w, w_scale, nullptr, nullptr, M, N, K, at, st);
     g.bias = bias;
     g.out = out;
-    const Fp8Plan plan = make_plan(M, N, K, false);
+    const Fp8Plan plan = make_plan(M, N, K, false, out_dtype != MIQ_F32);
     if (out_dtype == MIQ_F32) return run_product<MIQ_F32>(g, plan, at, st);
     if (out_dtype == MIQ_F16) return run_product<MIQ_F16>(g, plan, at, st);
     return run_product<MIQ_BF16>(g, plan, at, st);
 }
 
 extern "C" size_t miq_gated_fp8_workspace(int64_t M, int64_t N, int64_t K) {
-    return workspace_of("miq_gated_fp8_workspace", M, N, K, true);
+    return workspace_of("miq_gated_fp8_workspace", M, N, K, true, false);
 }
 
 extern "C" int miq_gated_fp8(const uint8_t* x, const float* x_scale, const uint8_t* w_gate, const float* gate_scale,
@@ -1062,7 +1093,7 @@ extern "C" int miq_gated_fp8(const uint8_t* x, const float* x_scale, const uint8
     const hipStream_t st = as_stream(stream);
     char* at = static_cast<char*>(workspace);
     Fp8Args g = make_args(x, x_scale, w_gate, gate_scale, w_up, up_scale, M, N, K, at, st);
-    const Fp8Plan plan = make_plan(M, N, K, true);
+    const Fp8Plan plan = make_plan(M, N, K, true, false);
     float* slabs = reinterpret_cast<float*>(at);
     return act == MIQ_ACT_SILU ? run_gated<MIQ_ACT_SILU>(g, plan, slabs, q, scale, st)
                                : run_gated<MIQ_ACT_GELU>(g, plan, slabs, q, scale, st);

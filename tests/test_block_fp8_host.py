@@ -71,7 +71,7 @@ def test_product_refusals():
         assert f(M=0) == 0 and f(N=0) == 0
     assert gemm(out=NULL) == -1 and gemm(dt=3) == -1 and gemm(dt=4) == -1 and gemm(out=P(4104)) == -2
     assert gated(act=2) == -1 and gated(q=NULL) == -1 and gated(su=NULL) == -1
-    assert L.miq_gemm_fp8_workspace(BIG, 4, 4) == 0 and L.miq_gated_fp8_workspace(4, -1, 4) == 0
+    assert L.miq_gemm_fp8_workspace(BIG, 4, 4, 0) == 0 and L.miq_gated_fp8_workspace(4, -1, 4) == 0
     for m in (1, 16, 100, 1000):
         if L.miq_gated_fp8_workspace(m, 512, 8192):
             assert gated(M=m, N=512, K=8192, size=16) == -3
