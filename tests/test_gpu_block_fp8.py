@@ -409,3 +409,64 @@ def test_same_call_same_bits(m):
         assert torch.equal(F.linear_fp8(xq, xs, *w8), a)
         c = F.gated_linear_fp8(xq, xs, *w8, *w8)
         assert torch.equal(c[0].view(torch.uint8), b[0].view(torch.uint8)) and torch.equal(c[1], b[1])
+
+
+# ---- layers ----------------------------------------------------------------------------------------------------------------
+
+def test_linear_layer(tmp_path):
+    """from_float, float and pair inputs, a state_dict round trip, and casts of the model that must not touch the weights."""
+    from quantization_amd import block_fp8 as F
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(520, 300)
+    layer = F.BlockFP8Linear.from_float(lin)
+    assert layer.weight.device.type == "cpu" and layer.weight.dtype == torch.float8_e4m3fn
+    rq, rs = R.quantize_weight(lin.weight.detach())
+    same_codes(layer.weight, rq)
+    assert torch.equal(layer.weight_scale, rs)
+    layer = torch.nn.Sequential(layer).to("cuda").to(torch.bfloat16)[0]
+    assert layer.weight.dtype == torch.float8_e4m3fn and layer.weight_scale.dtype == torch.float32 and layer.weight.is_cuda
+    assert layer.bias.dtype == torch.float32
+    x = rand(9, 520, torch.float32, 3).view(3, 3, 520).cuda()
+    y = layer(x)
+    assert y.dtype == torch.float32 and y.shape == (3, 3, 300)
+    want = F.linear_fp8(*F.quantize_blocks_fp8(x), layer.weight, layer.weight_scale, lin.bias.detach().cuda(), torch.float32)
+    assert torch.equal(y, want)
+    q, s = F.quantize_blocks_fp8(x)
+    assert torch.equal(layer((q, s)), want.to(torch.bfloat16))
+    torch.save(layer.state_dict(), tmp_path / "l.pt")
+    other = F.BlockFP8Linear.from_float(torch.nn.Linear(520, 300)).to("cuda")
+    other.load_state_dict(torch.load(tmp_path / "l.pt", weights_only=True))
+    assert torch.equal(other(x), y)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gated_mlp_layer(act):
+    from quantization_amd import block_fp8 as F
+    torch.manual_seed(1)
+    gate, up, down = torch.nn.Linear(384, 1000, bias=False), torch.nn.Linear(384, 1000, bias=False), torch.nn.Linear(1000, 384)
+    mlp = F.BlockFP8GatedMLP.from_float(gate, up, down, act).cuda().half()
+    x = rand(5, 384, torch.float16, 3).cuda()
+    h = F.gated_linear_fp8(*F.quantize_blocks_fp8(x), mlp.gate, mlp.gate_scale, mlp.up, mlp.up_scale, act)
+    want = F.linear_fp8(*h, mlp.down.weight, mlp.down.weight_scale, down.bias.detach().cuda(), torch.float16)
+    y = mlp(x)
+    assert y.dtype == torch.float16 and torch.equal(y, want)
+    assert torch.equal(mlp(F.quantize_blocks_fp8(x)).float(), F.linear_fp8(*h, mlp.down.weight, mlp.down.weight_scale, mlp.down.bias).float())
+    with pytest.raises(NotImplementedError):
+        F.BlockFP8GatedMLP.from_float(torch.nn.Linear(8, 8), up, down)
+    with pytest.raises(RuntimeError):
+        F.BlockFP8GatedMLP.from_float(gate, up, down, "relu")
+
+
+def test_another_device_current():
+    """Tensors on the current device's neighbour, where there is one; on one GPU: a stream that is not the default."""
+    from quantization_amd import block_fp8 as F
+    index = torch.cuda.device_count() - 1
+    x = rand(4, 256, torch.bfloat16, 1).to(f"cuda:{index}")
+    st = torch.cuda.Stream(index)
+    with torch.cuda.stream(st):
+        q, s = F.quantize_blocks_fp8(x)
+    st.synchronize()
+    assert q.device == x.device and torch.cuda.current_device() == 0
+    rq, rs = R.quantize_rows(x)
+    same_codes(q, rq)
+    assert torch.equal(s.cpu(), rs)
