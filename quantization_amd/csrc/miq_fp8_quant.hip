@@ -10,10 +10,8 @@ namespace {
 using namespace miq;
 
 // ---- activations: 1 x 128 ------------------------------------------------------------------------------------------
-// A workgroup of 16 sixteen-lane groups takes ROWS rows x (16 / ROWS) * PASSES blocks.
-constexpr int kQuantPasses = 4;
-
-template <int DT, bool VEC, int ROWS>
+// A workgroup of 16 sixteen-lane groups takes ROWS rows x (16 / ROWS) * kQuantPasses blocks.
+template <int DT, bool VEC, int ROWS, int kQuantPasses>
 __global__ __launch_bounds__(256) void quantize_blocks_kernel(const void* __restrict__ x, int64_t M, int64_t K, int64_t kblocks,
                                                               int64_t col_groups, uint8_t* __restrict__ q,
                                                               float* __restrict__ scale) {
@@ -268,20 +266,27 @@ extern "C" int miq_quantize_blocks_fp8(const void* x, int x_dtype, int64_t M, in
     MIQ_REQUIRE(aligned(x, elem_size(x_dtype)) && aligned(scale, 4), MIQ_EALIGN, "miq_quantize_blocks_fp8: misaligned pointer");
     const bool vec = K % 8 == 0 && aligned(x, 16) && aligned(q, 8);
     const int64_t kblocks = ceil_div(K, kBlockK);
-    const bool tall = M >= 16;
-    const int64_t col_groups = ceil_div(kblocks, (tall ? 1 : 16) * kQuantPasses);
+    // Sixteen rows of a block at a time where there are as many, so that their scales leave as one line; four blocks a thread
+    // in flight, or one where that would leave CUs idle (a few rows: the launch is all latency).
+    const bool tall = M >= 16, few = ceil_div(M, tall ? 16 : 1) * ceil_div(kblocks, tall ? 4 : 64) < 256;
+    const int64_t col_groups = ceil_div(kblocks, (tall ? 1 : 16) * (few ? 1 : 4));
     const int64_t grid = (tall ? ceil_div(M, 16) : M) * col_groups;
     MIQ_REQUIRE(grid <= kMaxGrid, MIQ_ERANGE, "miq_quantize_blocks_fp8: too many blocks");
     return for_dtype(x_dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        auto go = [&](auto v, auto rows) {
-            quantize_blocks_kernel<DT, decltype(v)::value, decltype(rows)::value>
+        auto go = [&](auto v, auto rows, auto passes) {
+            quantize_blocks_kernel<DT, decltype(v)::value, decltype(rows)::value, decltype(passes)::value>
                 <<<static_cast<unsigned>(grid), 256, 0, as_stream(stream)>>>(x, M, K, kblocks, col_groups, q, scale);
         };
-        using R16 = std::integral_constant<int, 16>;
-        using R1 = std::integral_constant<int, 1>;
-        if (vec) tall ? go(std::true_type{}, R16{}) : go(std::true_type{}, R1{});
-        else tall ? go(std::false_type{}, R16{}) : go(std::false_type{}, R1{});
+        auto shape = [&](auto v) {
+            std::integral_constant<int, 16> r16;
+            std::integral_constant<int, 1> one;
+            std::integral_constant<int, 4> four;
+            if (tall) few ? go(v, r16, one) : go(v, r16, four);
+            else few ? go(v, one, one) : go(v, one, four);
+        };
+        if (vec) shape(std::true_type{});
+        else shape(std::false_type{});
         return check_launch("quantize_blocks_kernel");
     });
 }

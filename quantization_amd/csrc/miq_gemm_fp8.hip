@@ -428,6 +428,15 @@ struct GatedOut {
 // GATED: the tile is 128 columns of both weights, a wave's column fragments 0, 1 the gate's and 2, 3 the up projection's
 // same 32 columns, so that a lane holds both factors of its outputs and the 128 columns are one block of the result.
 
+// f(FIRST), ..., f(END - 1) with the index a constant.
+template <int FIRST, int END, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (FIRST < END) {
+        f(std::integral_constant<int, FIRST>{});
+        static_for<FIRST + 1, END>(f);
+    }
+}
+
 template <int OUT, int ACT, bool NATIVE, int RF>
 __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut go) {
     constexpr bool GATED = ACT != kNoAct;
@@ -519,7 +528,9 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
         if constexpr (NATIVE) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
+                __builtin_amdgcn_s_setprio(1);   // (over the other wave of the SIMD, which scales or reads meanwhile)
                 c[j] = block_sum(wf[j], xf[i & 1]);
+                __builtin_amdgcn_s_setprio(0);
                 // column fragment j - 2 of this row fragment, or j + 2 of the one before
                 v4f& a = j < 2 ? acc[p][j + 2] : acc[i][j - 2];
 #pragma unroll
@@ -550,7 +561,6 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    using std::integral_constant;
     if (nt > 0) {
         stage(false, 0, x_slot(0));
         stage(true, 0, w_slot(0));
@@ -575,10 +585,7 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
             xf[0] = operand<NATIVE>(read(xt, 0));
 #pragma unroll
             for (int j = 0; j < 4; ++j) wf[j] = operand<NATIVE>(read(wt, w_row(j)));
-            rows_step(integral_constant<int, 0>{}, xt, sv0, sw0, sw1);
-            if constexpr (AS > 1) rows_step(integral_constant<int, 1>{}, xt, sv0, sw0, sw1);
-            if constexpr (AS > 2) rows_step(integral_constant<int, 2>{}, xt, sv0, sw0, sw1);
-            if constexpr (AS > 3) rows_step(integral_constant<int, 3>{}, xt, sv0, sw0, sw1);
+            static_for<0, AS>([&](auto i) { rows_step(i, xt, sv0, sw0, sw1); });
             if (group) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");   // x(t + 1), w(t + 1); x(t + 2) stays in flight
             barrier();
             // phase B
@@ -586,17 +593,7 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
             const int tn1 = t + 1 < nt ? t + 1 : t;
             sv0 = row_scales(tn1, 0);
             const uint32_t sv1_next = row_scales(tn1, 1);
-            if constexpr (RF == 2) rows_step(integral_constant<int, 1>{}, xt, sv1, sw0, sw1);
-            if constexpr (RF == 4) rows_step(integral_constant<int, 2>{}, xt, sv1, sw0, sw1);
-            if constexpr (RF == 4 || RF == 6) rows_step(integral_constant<int, 3>{}, xt, sv1, sw0, sw1);
-            if constexpr (RF >= 6) {
-                rows_step(integral_constant<int, 4>{}, xt, sv1, sw0, sw1);
-                rows_step(integral_constant<int, 5>{}, xt, sv1, sw0, sw1);
-            }
-            if constexpr (RF == 8) {
-                rows_step(integral_constant<int, 6>{}, xt, sv1, sw0, sw1);
-                rows_step(integral_constant<int, 7>{}, xt, sv1, sw0, sw1);
-            }
+            static_for<AS, RF>([&](auto i) { rows_step(i, xt, sv1, sw0, sw1); });
             sv1 = sv1_next;
             if (!group) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
             barrier();
@@ -920,12 +917,14 @@ int launch_tile(Fp8Args g, int splits, int products, hipStream_t st) {
     gemm_fp8_tile_kernel<BM, BN, WAVES_M, WAVES_N, STAGES, OUT, NATIVE><<<grid, 64 * WAVES_M * WAVES_N, kLds, st>>>(g);
     return check_launch("gemm_fp8_tile_kernel");
 }
-// NATIVE16: the products of a 16-bit output (the slabs' sums included) may use the 8-bit instruction.
+// NATIVE16: the products of a 16-bit output (the slabs' sums included) may use the 8-bit instruction.  Stages and waves as
+// measured: a ring of three K-tiles fits three workgroups a CU, one of four two (48x14336x4096 bf16 17.5 us against 19.3); 128 x
+// 128 tiles as eight waves of 32 x 64 (256x4096x14336 bf16 32.4 us, as four of 64 x 64 34.7, with a ring of three 49.7).
 template <int OUT, bool NATIVE16>
 int launch_tiles(const Fp8Plan& p, const Fp8Args& g, int products, hipStream_t st) {
-    if (p.bm == 32) return launch_tile<32, 64, 2, 2, 4, OUT, NATIVE16>(g, p.splits, products, st);
-    if (p.bm == 64) return launch_tile<64, 64, 2, 2, 4, OUT, NATIVE16>(g, p.splits, products, st);
-    return launch_tile<128, 128, 2, 2, 2, OUT, NATIVE16>(g, p.splits, products, st);
+    if (p.bm == 32) return launch_tile<32, 64, 2, 2, 3, OUT, NATIVE16>(g, p.splits, products, st);
+    if (p.bm == 64) return launch_tile<64, 64, 2, 2, 3, OUT, NATIVE16>(g, p.splits, products, st);
+    return launch_tile<128, 128, 4, 2, 2, OUT, NATIVE16>(g, p.splits, products, st);
 }
 
 template <int GROUPS, int OUT, int ACT>
