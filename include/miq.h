@@ -396,8 +396,8 @@ int miq_linear_dynamic_w8a8(const void* x, int x_dtype, const int8_t* W, int64_t
  *                                                            the conversion rounds half to even)
  * A value that is not finite becomes the NaN code and does not enter its block's maximum.
  *
- * Outputs must not overlap inputs.  A call whose launch would pass 2^32 threads returns MIQ_ERANGE (from 2^22 rows of more than
- * 8192 columns, 2^24 of fewer, or 2^24 blocks of 128 x 128). */
+ * Outputs must not overlap inputs.  A call whose launch would pass 2^32 threads returns MIQ_ERANGE (from 2^22 rows of a norm, or
+ * 2^24 workgroups of a quantizer). */
 
 /* Activations to codes: x [M,K] of x_dtype MIQ_F32 | MIQ_F16 | MIQ_BF16 -> q [M,K], scale [ceil(K/128), M]. */
 int miq_quantize_blocks_fp8(const void* x, int x_dtype, int64_t M, int64_t K, uint8_t* q, float* scale, void* stream);

@@ -66,16 +66,21 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t max_bits) {
 }
 
 // Eight consecutive elements of floating storage type DT as floats.  `n` of them are inside the row (the others read as
-// 0); VEC: the address is 16-byte aligned and n is 0 or 8.
-template <int DT, bool VEC>
+// 0); VEC: the address is 16-byte aligned and n is 0 or 8; NT: read once, kept out of the caches.
+template <bool NT>
+__device__ __forceinline__ u32x4 load16(const u32x4* p) {
+    if constexpr (NT) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+template <int DT, bool VEC, bool NT = true>
 __device__ __forceinline__ void load8(const void* base, int64_t index, int n, float (&f)[8]) {
     if constexpr (DT == MIQ_F32) {
         const float* p = static_cast<const float*>(base) + index;
         if constexpr (VEC) {
             u32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
             if (n > 0) {
-                a = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-                b = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p) + 1);
+                a = load16<NT>(reinterpret_cast<const u32x4*>(p));
+                b = load16<NT>(reinterpret_cast<const u32x4*>(p) + 1);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -90,7 +95,7 @@ __device__ __forceinline__ void load8(const void* base, int64_t index, int n, fl
         const uint16_t* p = static_cast<const uint16_t*>(base) + index;
         u32x4 v = {0, 0, 0, 0};
         if constexpr (VEC) {
-            if (n > 0) v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+            if (n > 0) v = load16<NT>(reinterpret_cast<const u32x4*>(p));
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -115,7 +120,7 @@ __device__ __forceinline__ void load8(const void* base, int64_t index, int n, fl
 template <bool VEC>
 __device__ __forceinline__ void store8_codes(uint8_t* q, int64_t index, int n, const uint32_t (&c)[2]) {
     if constexpr (VEC) {
-        if (n > 0) *reinterpret_cast<u32x2*>(q + index) = u32x2{c[0], c[1]};
+        if (n > 0) __builtin_nontemporal_store(u32x2{c[0], c[1]}, reinterpret_cast<u32x2*>(q + index));
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
