@@ -132,6 +132,9 @@ __device__ __forceinline__ void store4(void* out, int64_t i, int n, bool vec, v4
     }
 }
 
+// Memory requests before this stay before it, those after it after: the counted waits below depend on the order of issue.
+__device__ __forceinline__ void keep_order() { asm volatile("" ::: "memory"); }
+
 // Fills one LDS tile with 16-byte LDS-DMA: K-tile kt of the ROWS rows at `rows`, `nrows` of which exist (the others, and
 // columns past K, read as zeros).
 template <int ROWS, int NWAVES>
@@ -238,7 +241,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
         const int k = kt < kt1 ? kt : g.kblocks;
         stage_rows<BM, NWAVES>(xrows, mrows, g.K, k, buf, wave, lane);
         stage_rows<BN, NWAVES>(wrows, nrows, g.K, k, buf + BM * kTileK, wave, lane);
-        const __amdgpu_buffer_rsrc_t rs = make_rsrc(g.xs + static_cast<int64_t>(kt < kt1 ? kt : kt0) * g.M + m0, static_cast<uint32_t>(mrows) * 4);
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(g.xs + static_cast<int64_t>(kt < kt1 ? kt : kt0) * g.M + m0, kt < kt1 ? static_cast<uint32_t>(mrows) * 4 : 0);
 #pragma unroll
         for (int i = 0; i < kScaleLoads; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(buf + kRowBytes + (wave * kScaleLoads + i) * 256), 4,
@@ -276,12 +279,15 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
             constexpr int kKeep = ((BM / 8 + BN / 8) / NWAVES + kScaleLoads) * (STAGES - 2);
             static_assert(kKeep <= 63, "vmcnt is a 6-bit counter");
 #pragma unroll
-            for (int t = 0; t < STAGES - 1; ++t) stage(smem + t * STAGE, kt0 + t);
+            for (int t = 0; t < STAGES - 1; ++t) {
+                stage(smem + t * STAGE, kt0 + t);
+                keep_order();
+            }
             int slot = 0, fill = STAGES - 1;
             for (int kt = kt0; kt < kt1; ++kt) {
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kKeep) : "memory");
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kKeep) : "memory");
                 __builtin_amdgcn_s_barrier();   // K-tile kt is there for every wave; every wave has read kt - 1
-                asm volatile("" ::: "memory");
+                keep_order();
                 stage(smem + fill * STAGE, kt + STAGES - 1);
                 multiply(smem + slot * STAGE, kt);
                 slot = slot + 1 == STAGES ? 0 : slot + 1;
@@ -360,7 +366,7 @@ __global__ __launch_bounds__(64 * kWaves) void gemm_fp8_rows16_kernel(Fp8Args g)
             for (int j = 0; j < GROUPS; ++j) s.w[j].c[h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw[j], off, 0, 0));
             s.x.c[h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 0, 0));
         }
-        const __amdgpu_buffer_rsrc_t rs = make_rsrc(g.xs + static_cast<int64_t>(in ? kt : kt0) * g.M, static_cast<uint32_t>(g.M) * 4);
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(g.xs + static_cast<int64_t>(in ? kt : 0) * g.M, in ? static_cast<uint32_t>(g.M) * 4 : 0);
         s.s = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, (lane & 15) * 4, 0, 0));
     };
 
@@ -421,7 +427,7 @@ struct GatedOut {
 //     after barrier 2t + 1 the rows x(t - 1) are read by nobody any more:  DMA of x(t + 2) into their slot (three slots)
 //     after barrier 2t     the rows w(t - 2 + 1) likewise:                 DMA of w(t + 1) (two slots)
 //     before barrier 2t    every wave has waited for its share of x(t) and w(t), issued three and two phases earlier; the
-//                          four pieces of x(t + 1) and two loads of scales may still be in flight
+//                          four pieces of x(t + 1) may still be in flight
 // which fills the CU's 160 KiB of LDS with 32 KiB slots.  K-tiles past the end are requested out of range (zeros, no memory
 // traffic), so that every wave issues the same number of pieces.
 //
@@ -540,8 +546,10 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
                 __builtin_amdgcn_sched_barrier(0);
             }
         } else {
-            if (i > 0) xf[0] = widen(raw);
-            if (i < RF - 1) raw = read(xt, (i + 1) * 16);
+            if (i > 0) {
+                xf[0] = widen(raw);
+                if (i < RF - 1) raw = read(xt, (i + 1) * 16);
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -561,12 +569,18 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
+    // Every request of the four youngest pieces' phase or later may be in flight, everything older has landed; and this wave's
+    // LDS reads have returned (the slots that they read are written after the barrier).
+    auto wait_all_but_one_slot = [] { asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory"); };
+    auto wait_reads = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
     if (nt > 0) {
+        uint32_t sv0 = row_scales(0, 0), sv1 = row_scales(0, 1);
+        keep_order();
         stage(false, 0, x_slot(0));
         stage(true, 0, w_slot(0));
+        keep_order();
         stage(false, 1, x_slot(1));
-        uint32_t sv0 = row_scales(0, 0), sv1 = row_scales(0, 1);
-        asm volatile("s_waitcnt vmcnt(6)" ::: "memory");   // x(0), w(0)
+        wait_all_but_one_slot();   // x(0), w(0)
         barrier();
         int group = wm;
         if (group == 1) {
@@ -585,17 +599,21 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
             xf[0] = operand<NATIVE>(read(xt, 0));
 #pragma unroll
             for (int j = 0; j < 4; ++j) wf[j] = operand<NATIVE>(read(wt, w_row(j)));
+            if constexpr (!NATIVE) raw = read(xt, 16);
             static_for<0, AS>([&](auto i) { rows_step(i, xt, sv0, sw0, sw1); });
-            if (group) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");   // x(t + 1), w(t + 1); x(t + 2) stays in flight
+            if (group) wait_all_but_one_slot();   // x(t + 1), w(t + 1); x(t + 2) stays in flight
+            else wait_reads();
             barrier();
-            // phase B
-            stage(group != 0, t + 2, group ? w_slot(t + 2) : x_slot(ahead));
+            // phase B: the next scales are requested ahead of the pieces, so that the wait behind these covers them
             const int tn1 = t + 1 < nt ? t + 1 : t;
             sv0 = row_scales(tn1, 0);
             const uint32_t sv1_next = row_scales(tn1, 1);
+            keep_order();
+            stage(group != 0, t + 2, group ? w_slot(t + 2) : x_slot(ahead));
             static_for<AS, RF>([&](auto i) { rows_step(i, xt, sv1, sw0, sw1); });
             sv1 = sv1_next;
-            if (!group) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+            if (group) wait_reads();
+            else wait_all_but_one_slot();
             barrier();
         }
         if (wm == 0) barrier();   // every wave executes the same number of barriers

@@ -411,6 +411,47 @@ def test_same_call_same_bits(m):
         assert torch.equal(c[0].view(torch.uint8), b[0].view(torch.uint8)) and torch.equal(c[1], b[1])
 
 
+# ---- random shapes, every kernel that a size can choose ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("seed", range(8))
+def test_random_shapes(seed):
+    """Sizes spread over their logarithm; codes by the kernels' own quantizer (checked above, bit for bit), products on the
+    GPU in float64."""
+    import random
+    from quantization_amd import block_fp8 as F
+    rng = random.Random(seed)
+
+    def size(lo, hi):
+        return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+    for _ in range(10):
+        m, n = size(1, 1200), size(1, 9000)
+        step = rng.choice([1, 16, 128])
+        k = max(step, size(1, 6000) // step * step)
+        out, act = rng.choice(FLOATS), rng.choice(["silu", "gelu"])
+        xq, xs = F.quantize_blocks_fp8(rand(m, k, torch.float32, m).cuda())
+        w = [F.quantize_weight_fp8((rand(n, k, torch.float32, n + j) / math.sqrt(k)).cuda()) for j in range(2)]
+        bk, bn = torch.arange(k, device="cuda") // 128, torch.arange(n, device="cuda") // 128
+        x = xq.double() * xs.double().t()[:, bk]
+        ws = [q.double() * s.double()[bn][:, bk] for q, s in w]
+        ref, mag = x @ ws[0].t(), x.abs() @ ws[0].abs().t()
+        y = F.linear_fp8(xq, xs, *w[0], None, out)
+        err = R.product_error(mag, k) + dropped(out, m) * mag
+        tol = err + torch.finfo(out).eps / 2 * (ref.abs() + err) + torch.finfo(out).smallest_normal * torch.finfo(out).eps
+        fits = ref.abs() < torch.finfo(out).max * 0.99
+        off = (y.double() - ref).abs()
+        assert bool((off <= tol)[fits].all()), (m, n, k, out, float((off / tol)[fits].max()))
+        u, umag = x @ ws[1].t(), x.abs() @ ws[1].abs().t()
+        a = R.act(ref, act)
+        da = 1.13 * R.product_error(mag, k) + 8 * 2.0 ** -23 * ref.abs()
+        h = a * u
+        dh = da * (u.abs() + R.product_error(umag, k)) + a.abs() * R.product_error(umag, k) + 2.0 ** -23 * h.abs()
+        q, s = F.gated_linear_fp8(xq, xs, *w[0], *w[1], act)
+        try:
+            R.check_codes_of(q, s, h.cpu(), dh.cpu())
+        except AssertionError as e:
+            raise AssertionError(f"gated {m} x {n} x {k} {act}: {e}") from None
+
+
 # ---- layers ----------------------------------------------------------------------------------------------------------------
 
 def test_linear_layer(tmp_path):
