@@ -299,19 +299,45 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
 
     // A fragment's results: 4 * (lane >> 4) + register -> column n, lane & 15 -> row m.
     const int cols = g.kt_per_split ? g.pitch : g.N;   // of a row of `out`
-    const bool vec = (cols & 3) == 0;
+    v4f b[FN];
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
         const int n = n0 + wn * WN + j * 16 + (lane >> 4) * 4;
-        if (n >= cols) continue;
-        v4f b = {0.f, 0.f, 0.f, 0.f};
-        if (g.bias && !g.kt_per_split)
-            for (int e = 0; e < 4; ++e)
-                if (n + e < g.N) b[e] = g.bias[n + e];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[j][e] = g.bias && !g.kt_per_split && n + e < g.N ? g.bias[n + e] : 0.f;
+    }
+    if ((cols & 3) == 0) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int n = n0 + wn * WN + j * 16 + (lane >> 4) * 4;
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                const int64_t m = m0 + wm * WM + i * 16 + (lane & 15);
+                if (n < cols && m < g.M) store4<OUT>(out, m * cols + n, cols - n, true, acc[i][j] + b[j]);
+            }
+        }
+    } else {
+        // Rows that start anywhere: a row fragment's 16 x WN through LDS, then 64 / WN rows an instruction, a column a lane (an
+        // element at a time from where the results lie, 1 to 2 TB/s: 2312x2166x128 bf16 15.8 us, this way 9.1).
+        constexpr int kPitch = WN + 4;
+        static_assert(NWAVES * 16 * kPitch * 4 <= STAGES * STAGE, "fits the ring");
+        __syncthreads();   // every wave has read its last K-tile
+        float* const rows = reinterpret_cast<float*>(smem) + wave * (16 * kPitch);
+        const int n = n0 + wn * WN + lane % WN;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
-            const int64_t m = m0 + wm * WM + i * 16 + (lane & 15);
-            if (m < g.M) store4<OUT>(out, m * cols + n, cols - n, vec, acc[i][j] + b);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) *reinterpret_cast<v4f*>(rows + (lane & 15) * kPitch + j * 16 + (lane >> 4) * 4) = acc[i][j] + b[j];
+            wave_lds_order();
+            const int64_t m = m0 + wm * WM + i * 16 + lane / WN;
+            constexpr int kStep = 64 / WN;
+            float v[16 / kStep];
+#pragma unroll
+            for (int r = 0; r < 16; r += kStep) v[r / kStep] = rows[(r + lane / WN) * kPitch + lane % WN];
+            wave_lds_order();
+#pragma unroll
+            for (int r = 0; r < 16; r += kStep)
+                if (n < cols && m + r < g.M) store_value<OUT>(out, (m + r) * cols + n, v[r / kStep]);
         }
     }
 }
@@ -847,7 +873,7 @@ size_t padded_bytes(int64_t M, int64_t N, int64_t weights, int64_t K) {
 // What a product is cut into: which kernel, how K is split, and how much workspace that needs behind the padded operands.
 struct Fp8Plan {
     int big;         // rows of the large kernel's tile, 256, 192, 128 or 64; 0: not that kernel
-    int bm;          // rows of the tile kernel's tile; 0: the kernel for at most 16 rows
+    int bm;          // rows of the tile kernel's tile, 128, 64 or 32; 0: the kernel for at most 16 rows
     int splits;      // slices of K; 1: none
     int kt_per_split;
     size_t slabs;    // bytes of fp32 slabs
@@ -855,73 +881,98 @@ struct Fp8Plan {
 
 constexpr int64_t kCus = 256;
 
-// Above 16 rows either kernel can run a product; the one with the smaller estimate does.
+// Above 16 rows the large kernel and the tile kernel, the latter with tiles of three heights and K in any number of slices, can
+// all run a product: the one with the smallest estimate does.  The estimates' constants are us, fitted to 150 shapes from
+// 17x64x128 to 4000x28672x28672 on every variant (the estimates are within 12% of the times, the choice within 2% of the best
+// variant's on average).  E.g. 512x2048x2048 bf16: large kernel 19.2 (64 rows), 128-row tiles 16.6, 64 9.1, 64 in two slices 14.4;
+// 254x354x2560 bf16 23.5, 128-row tiles in two slices 13.6, 32-row tiles whole 8.5, in four slices 7.5; gated 2785x669x10032 163
+// (128 rows), 128-row tiles in two slices 123, in four 113; gated 2773x5456x224 34.6 (256 rows), 128-row tiles 56.
 //
-// The large kernel has one workgroup a CU: a launch takes as many rounds as its tiles need, and a round a time for each
-// K-tile that hardly depends on the rest.  Measured, us a K-tile and round for tiles of 256, 192, 128, 64 rows: bf16 form
-// (fp32 out, gated) 3.3 2.7 2.15 1.6, 8-bit form 1.8 1.5 1.2 1.0; a few us of prologue and epilogue on top.  The tile kernel
-// fills the chip with small tiles or slices of K and is bound by its own vector and matrix work (128 x 128 tiles 0.75 and
-// 1.0 PFLOP/s, thin tiles 0.55 and 0.9) or by the weight's stream (about 5 TB/s), on top of 8 us of launches.  E.g., us on the
-// tile kernel | the large one: 1024x4096x4096 bf16 37 | 33 (64 rows), 2048x4096x4096 bf16 73 | 41 (128), gated 256x14336x4096
-// 78 | 72 (128), gated 512x4096x4096 46 | 52, 512x4096x4096 bf16 27 | 33, fp32 1024x4096x4096 47 | 51.
-struct BigChoice {
-    int rows;
-    double us;
+// The large kernel has one workgroup a CU: it takes as many rounds as its tiles need, each a time a K-tile and a prologue and
+// epilogue.
+struct Fit {
+    double k_tile, fixed;
 };
-BigChoice best_big(int64_t M, int64_t N, int64_t nt, bool gated, bool native) {
-    static constexpr int kTall[4] = {256, 192, 128, 64};
-    static constexpr double kUs[2][4] = {{3.3, 2.7, 2.15, 1.6}, {1.8, 1.5, 1.2, 1.0}};
-    const int64_t across = ceil_div(N, gated ? 128 : 256);
-    BigChoice best{256, 1e30};
-    for (int i = 0; i < 4; ++i) {
-        const double rounds = static_cast<double>(ceil_div(ceil_div(M, kTall[i]) * across, kCus));
-        const double us = rounds * (kUs[native][i] * static_cast<double>(nt) + 4.0);
-        if (us < best.us) best = {kTall[i], us};
-    }
-    best.us += 4.0;
-    return best;
+double big_us(int i, int64_t M, int64_t N, int64_t nt, bool gated, bool native) {
+    static constexpr Fit kFit[2][4] = {{{2.90, 13.6}, {2.37, 11.4}, {1.91, 8.8}, {1.46, 5.7}},     // bf16 form: 256 to 64 rows
+                                       {{1.48, 10.9}, {1.29, 8.8}, {1.06, 6.8}, {0.94, 5.0}}};   // 8-bit form
+    const int64_t tiles = ceil_div(M, 256 - 64 * i) * ceil_div(N, gated ? 128 : 256);
+    return static_cast<double>(ceil_div(tiles, kCus)) * (kFit[native][i].k_tile * static_cast<double>(nt) + kFit[native][i].fixed);
 }
-double tile_us(int64_t M, int64_t N, int64_t K, bool gated, bool native) {
-    const double flops = (gated ? 4.0 : 2.0) * static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
-    const double rate = M > 128 ? (native ? 1.0e9 : 0.75e9) : (native ? 0.9e9 : 0.55e9);   // a us
-    const double work = flops / rate, stream = (gated ? 2.0 : 1.0) * static_cast<double>(N) * static_cast<double>(K) / 5.0e6;
-    return 8.0 + (work > stream ? work : stream);
+// The tile kernel: `groups` workgroups of `kt` K-tiles each.  A workgroup alone on its CU takes `alone` a K-tile (a fetch and its
+// own matrix work), a full CU `full` for each workgroup's; never less than the weight's stream.  A second launch adds up slabs.
+struct TileFit {
+    int rows, resident;   // ... and workgroups a CU holds
+    double alone[2], full[2], fixed[2];   // bf16 form, 8-bit form
+};
+constexpr TileFit kTiles[3] = {{32, 4, {0.35, 0.25}, {0.23, 0.20}, {4.0, 3.3}},
+                               {64, 3, {0.45, 0.33}, {0.34, 0.29}, {4.1, 3.6}},
+                               {128, 2, {1.0, 0.89}, {0.85, 0.72}, {5.6, 4.0}}};
+double tile_us(const TileFit& t, int64_t groups, int64_t kt, bool native) {
+    const int64_t deep = ceil_div(groups, kCus);   // workgroups of the busiest CU
+    const double alone = t.alone[native] * static_cast<double>(ceil_div(deep, t.resident)), full = t.full[native] * static_cast<double>(deep);
+    return t.fixed[native] + static_cast<double>(kt) * (alone > full ? alone : full);
 }
 
 Fp8Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated, bool native) {
     Fp8Plan p{};
     p.splits = 1;
     const int64_t nt = ceil_div(K, kTileK);
-    if (M > 16) {
-        const BigChoice big = best_big(M, N, nt, gated, native);
-        if (M > 4096 || big.us <= tile_us(M, N, K, gated, native)) {
-            p.big = big.rows;
-            return p;
+    const int64_t slab = 4 * M * round_up(N, 8);
+    if (M <= 16) {
+        // A slice of K to every eighth workgroup's worth of K-tiles where the columns give few workgroups and K is long enough to
+        // pay for the second launch: 1x512x28672 18.3 us whole, 8.0 in eight slices, 1x512x14336 11.2 and 6.6 (and 4 us more of
+        // the host), 1x2048x8192 7.4 and 8.3.  A gated product has its second launch anyway and would have a third.
+        const int64_t groups = ceil_div(N, 16);
+        if (!gated && groups < 192 && nt >= 128) {
+            int64_t splits = kCus / groups;
+            if (splits > nt / 8) splits = nt / 8;
+            if (splits > 32) splits = 32;
+            p.kt_per_split = static_cast<int>(ceil_div(nt, splits));
+            p.splits = static_cast<int>(ceil_div(nt, p.kt_per_split));
+        }
+        p.slabs = gated ? static_cast<size_t>(4 * M * N) : p.splits > 1 ? static_cast<size_t>(slab) * p.splits : 0;   // gated: act(g) * u
+        return p;
+    }
+    double best = 1e30;
+    for (int i = 0; i < 4; ++i) {
+        const double us = big_us(i, M, N, nt, gated, native);
+        if (us < best) {
+            best = us;
+            p.big = 256 - 64 * i;
         }
     }
-    int64_t groups, want;
-    if (M <= 16) {
-        groups = ceil_div(N, 16);
-        want = 256;
-    } else {
-        p.bm = M <= 32 ? 32 : M <= 128 ? 64 : 128;
-        groups = ceil_div(M, p.bm) * ceil_div(N, p.bm == 128 ? 128 : 64) * (gated ? 2 : 1);
-        want = p.bm == 128 ? 512 : 768;
+    const int products = gated ? 2 : 1;
+    const double stream = static_cast<double>(products * N * K) / 4.5e6;   // us, at 4.5 TB/s
+    constexpr int64_t kMostSlabs = int64_t{1} << 28;
+    static constexpr int kSlices[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+    for (const TileFit& t : kTiles) {
+        const int64_t tiles = ceil_div(M, t.rows) * ceil_div(N, t.rows == 128 ? 128 : 64) * products;
+        for (const int s : kSlices) {
+            if (s > 1 && (s > nt / 2 || tiles * s > 6 * kCus)) break;
+            const int64_t kt = ceil_div(nt, s), slices = nt > 0 ? ceil_div(nt, kt) : 1;
+            double us = tile_us(t, tiles * slices, kt, native);
+            if (us < stream) us = stream;
+            if (slices > 1 || gated) {
+                const int64_t bytes = products * slices * slab;
+                if (bytes > kMostSlabs) break;
+                us += 4.0 + static_cast<double>(bytes) / 3.0e6;   // written and read
+            }
+            if (us >= best) continue;
+            best = us;
+            p.big = 0;
+            p.bm = t.rows;
+            p.splits = static_cast<int>(slices);
+            p.kt_per_split = static_cast<int>(slices > 1 || gated ? (kt > 0 ? kt : 1) : 0);   // gated: one slab a weight at least
+        }
     }
-    // Split K where the tiles alone leave CUs idle, into slices of at least eight K-tiles.
-    int64_t splits = groups < want * 3 / 4 ? want / groups : 1;
-    if (splits > nt / 8) splits = nt / 8;
-    if (splits < 1) splits = 1;
-    if (splits > 32) splits = 32;
-    if (splits > 1) {
-        p.kt_per_split = static_cast<int>(ceil_div(nt, splits));
-        p.splits = static_cast<int>(ceil_div(nt, p.kt_per_split));
+    if (p.big) {
+        p.bm = 0;
+        p.splits = 1;
+        p.kt_per_split = 0;
+    } else if (gated || p.splits > 1) {
+        p.slabs = static_cast<size_t>(products * p.splits * slab);
     }
-    const int64_t slab = 4 * M * round_up(N, 8);
-    if (gated && p.bm == 0 && p.splits == 1) p.slabs = static_cast<size_t>(4 * M * N);   // act(g) * u
-    else if (gated) p.slabs = static_cast<size_t>(2 * slab) * p.splits;
-    else if (p.splits > 1) p.slabs = static_cast<size_t>(slab) * p.splits;
-    if (gated && p.splits == 1 && p.bm != 0) p.kt_per_split = static_cast<int>(nt > 0 ? nt : 1);   // one slab a weight
     return p;
 }
 
@@ -1043,19 +1094,11 @@ int run_gated(Fp8Args g, const Fp8Plan& p, float* slabs, uint8_t* q, float* scal
     if (p.big) return launch_big<MIQ_F32, ACT, false>(p, g, {q, scale}, st);
     g.out = slabs;
     g.kt_per_split = p.kt_per_split;
-    if (p.bm == 0 && p.splits == 1) {
+    if (p.bm == 0) {
         if (int rc = launch_rows16<2, MIQ_F32, ACT>(p, g, st)) return rc;
         return miq_quantize_blocks_fp8(slabs, MIQ_F32, g.M, g.N, q, scale, st);
     }
-    if (p.bm == 0) {   // both weights' slabs, one launch each
-        if (int rc = launch_rows16<1, MIQ_F32, kNoAct>(p, g, st)) return rc;
-        g.w[0] = g.w[1];
-        g.ws[0] = g.ws[1];
-        g.out = slabs + static_cast<int64_t>(p.splits) * g.M * g.pitch;
-        if (int rc = launch_rows16<1, MIQ_F32, kNoAct>(p, g, st)) return rc;
-    } else if (int rc = launch_tiles<MIQ_F32, false>(p, g, 2, st)) {
-        return rc;
-    }
+    if (int rc = launch_tiles<MIQ_F32, false>(p, g, 2, st)) return rc;
     const int nblocks = static_cast<int>(ceil_div(g.N, 128));
     gated_join_kernel<ACT><<<static_cast<unsigned>(ceil_div(g.M * nblocks, 16)), 256, 0, st>>>(slabs, p.splits, g, nblocks, q, scale);
     return check_launch("gated_join_kernel");
@@ -1078,13 +1121,13 @@ extern "C" int miq_gemm_fp8(const uint8_t* x, const float* x_scale, const uint8_
     MIQ_REQUIRE(aligned(x_scale, 4) && aligned(w_scale, 4) && aligned(bias, 4) && aligned(out, 16), MIQ_EALIGN,
                 "miq_gemm_fp8: scales and bias must be 4-byte, out 16-byte aligned");
     MIQ_REQUIRE(K % kChunk != 0 || (aligned(x, 16) && aligned(w, 16)), MIQ_EALIGN, "miq_gemm_fp8: x and w must be 16-byte aligned");
-    if (int rc = check_workspace("miq_gemm_fp8", miq_gemm_fp8_workspace(M, N, K, out_dtype), workspace, workspace_bytes)) return rc;
+    const Fp8Plan plan = make_plan(M, N, K, false, out_dtype != MIQ_F32);
+    if (int rc = check_workspace("miq_gemm_fp8", padded_bytes(M, N, 1, K) + plan.slabs, workspace, workspace_bytes)) return rc;
     const hipStream_t st = as_stream(stream);
     char* at = static_cast<char*>(workspace);
     Fp8Args g = make_args(x, x_scale, w, w_scale, nullptr, nullptr, M, N, K, at, st);
     g.bias = bias;
     g.out = out;
-    const Fp8Plan plan = make_plan(M, N, K, false, out_dtype != MIQ_F32);
     if (out_dtype == MIQ_F32) return run_product<MIQ_F32>(g, plan, at, st);
     if (out_dtype == MIQ_F16) return run_product<MIQ_F16>(g, plan, at, st);
     return run_product<MIQ_BF16>(g, plan, at, st);
@@ -1106,11 +1149,11 @@ extern "C" int miq_gated_fp8(const uint8_t* x, const float* x_scale, const uint8
                 "miq_gated_fp8: scales must be 4-byte, q 16-byte aligned");
     MIQ_REQUIRE(K % kChunk != 0 || (aligned(x, 16) && aligned(w_gate, 16) && aligned(w_up, 16)), MIQ_EALIGN,
                 "miq_gated_fp8: x and the weights must be 16-byte aligned");
-    if (int rc = check_workspace("miq_gated_fp8", miq_gated_fp8_workspace(M, N, K), workspace, workspace_bytes)) return rc;
+    const Fp8Plan plan = make_plan(M, N, K, true, false);
+    if (int rc = check_workspace("miq_gated_fp8", padded_bytes(M, N, 2, K) + plan.slabs, workspace, workspace_bytes)) return rc;
     const hipStream_t st = as_stream(stream);
     char* at = static_cast<char*>(workspace);
     Fp8Args g = make_args(x, x_scale, w_gate, gate_scale, w_up, up_scale, M, N, K, at, st);
-    const Fp8Plan plan = make_plan(M, N, K, true, false);
     float* slabs = reinterpret_cast<float*>(at);
     return act == MIQ_ACT_SILU ? run_gated<MIQ_ACT_SILU>(g, plan, slabs, q, scale, st)
                                : run_gated<MIQ_ACT_GELU>(g, plan, slabs, q, scale, st);
