@@ -13,6 +13,8 @@
 // operands that is 3e-5 of the result, a hundred times an fp32 sum's error.  v_mfma_f32_16x16x32_bf16 keeps 24 bits
 // throughout (1e-8 on the same operands), and e4m3 widens to bf16 exactly (v_cvt_scalef32_pk_bf16_fp8, two codes an
 // instruction), at half the rate.
+#include <cmath>
+
 #include "miq_fp8.h"
 #include "miq_gemm_core.h"
 
@@ -882,36 +884,46 @@ struct Fp8Plan {
 constexpr int64_t kCus = 256;
 
 // Above 16 rows the large kernel and the tile kernel, the latter with tiles of three heights and K in any number of slices, can
-// all run a product: the one with the smallest estimate does.  The estimates' constants are us, fitted to 150 shapes from
-// 17x64x128 to 4000x28672x28672 on every variant (the estimates are within 12% of the times, the choice within 2% of the best
-// variant's on average).  E.g. 512x2048x2048 bf16: large kernel 19.2 (64 rows), 128-row tiles 16.6, 64 9.1, 64 in two slices 14.4;
-// 254x354x2560 bf16 23.5, 128-row tiles in two slices 13.6, 32-row tiles whole 8.5, in four slices 7.5; gated 2785x669x10032 163
-// (128 rows), 128-row tiles in two slices 123, in four 113; gated 2773x5456x224 34.6 (256 rows), 128-row tiles 56.
-//
-// The large kernel has one workgroup a CU: it takes as many rounds as its tiles need, each a time a K-tile and a prologue and
-// epilogue.
-struct Fit {
-    double k_tile, fixed;
+// all run a product: the one with the smallest estimate does.  The estimates' constants are us, fitted to the times of every
+// variant on 227 shapes from 17x64x128 to 8192x28672x28672 (the estimates are within 12% of the times, the choice within 3% of
+// the best variant's time on average).  E.g. 512x2048x2048 bf16: large kernel 19.2 (64 rows), 128-row tiles 16.6, 64 9.1, 64 in
+// two slices 14.4; 254x354x2560 bf16 23.5, 128-row tiles in two slices 13.6, 32-row tiles whole 8.5, in four slices 7.5; gated
+// 2785x669x10032 163 (128 rows), 128-row tiles in two slices 123, in four 113; gated 2773x5456x224 34.6 (256 rows), 128-row tiles
+// 56; fp32 1000x10001x4000 91 (192 rows), 107 (256), 128-row tiles 100.
+struct BigFit {
+    double k_tile, round;
 };
-double big_us(int i, int64_t M, int64_t N, int64_t nt, bool gated, bool native) {
-    static constexpr Fit kFit[2][4] = {{{2.90, 13.6}, {2.37, 11.4}, {1.91, 8.8}, {1.46, 5.7}},     // bf16 form: 256 to 64 rows
-                                       {{1.48, 10.9}, {1.29, 8.8}, {1.06, 6.8}, {0.94, 5.0}}};   // 8-bit form
-    const int64_t tiles = ceil_div(M, 256 - 64 * i) * ceil_div(N, gated ? 128 : 256);
-    return static_cast<double>(ceil_div(tiles, kCus)) * (kFit[native][i].k_tile * static_cast<double>(nt) + kFit[native][i].fixed);
+// `work` us of the workgroups' K-tiles while `weights` bytes stream at `rate` bytes a ps: the larger, somewhat more where they
+// are near each other.
+double overlapped_us(double work, double weights, double rate) {
+    const double stream = weights / (rate * 1e6), w2 = work * work, s2 = stream * stream;
+    return std::sqrt(std::sqrt(w2 * w2 + s2 * s2));
 }
-// The tile kernel: `groups` workgroups of `kt` K-tiles each.  A workgroup alone on its CU takes `alone` a K-tile (a fetch and its
-// own matrix work), a full CU `full` for each workgroup's; never less than the weight's stream.  A second launch adds up slabs.
+// One workgroup a CU: as many rounds as the tiles need, each a time a K-tile and a prologue and epilogue.
+double big_us(int i, int64_t M, int64_t N, int64_t nt, double weights, bool gated, bool native) {
+    static constexpr BigFit kFit[2][4] = {{{3.05, 12.9}, {2.46, 10.7}, {1.94, 8.5}, {1.50, 5.0}},   // bf16 form: 256 to 64 rows
+                                          {{1.72, 9.0}, {1.34, 9.1}, {1.12, 6.0}, {1.03, 3.9}}};    // 8-bit form
+    const BigFit& f = kFit[native][i];
+    const int64_t tiles = ceil_div(M, 256 - 64 * i) * ceil_div(N, gated ? 128 : 256);
+    return 1.0 + overlapped_us(static_cast<double>(ceil_div(tiles, kCus)) * (f.k_tile * static_cast<double>(nt) + f.round), weights, 2.8);
+}
+// `groups` workgroups of `kt` K-tiles each, `resident` on a CU.  A workgroup alone on its CU takes `alone` a K-tile (a fetch and
+// its own matrix work), a full CU `full` for each workgroup's; `stream` is the rate of the weights' stream, bytes a ps.
 struct TileFit {
-    int rows, resident;   // ... and workgroups a CU holds
-    double alone[2], full[2], fixed[2];   // bf16 form, 8-bit form
+    double fixed, alone, full, stream;
 };
-constexpr TileFit kTiles[3] = {{32, 4, {0.35, 0.25}, {0.23, 0.20}, {4.0, 3.3}},
-                               {64, 3, {0.45, 0.33}, {0.34, 0.29}, {4.1, 3.6}},
-                               {128, 2, {1.0, 0.89}, {0.85, 0.72}, {5.6, 4.0}}};
-double tile_us(const TileFit& t, int64_t groups, int64_t kt, bool native) {
+struct Tile {
+    int rows, resident;
+    TileFit fit[2];   // bf16 form, 8-bit form
+};
+constexpr Tile kTiles[3] = {{32, 4, {{3.85, 0.34, 0.24, 5.25}, {3.2, 0.26, 0.20, 5.25}}},
+                            {64, 3, {{4.1, 0.445, 0.345, 5.25}, {3.5, 0.34, 0.283, 5.25}}},
+                            {128, 2, {{5.7, 1.08, 0.927, 4.45}, {4.4, 0.95, 0.69, 4.0}}}};
+double tile_us(const Tile& t, int64_t groups, int64_t kt, double weights, bool native) {
+    const TileFit& f = t.fit[native];
     const int64_t deep = ceil_div(groups, kCus);   // workgroups of the busiest CU
-    const double alone = t.alone[native] * static_cast<double>(ceil_div(deep, t.resident)), full = t.full[native] * static_cast<double>(deep);
-    return t.fixed[native] + static_cast<double>(kt) * (alone > full ? alone : full);
+    const double alone = f.alone * static_cast<double>(ceil_div(deep, t.resident)), full = f.full * static_cast<double>(deep);
+    return f.fixed + overlapped_us(static_cast<double>(kt) * (alone > full ? alone : full), weights, f.stream);
 }
 
 Fp8Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated, bool native) {
@@ -934,29 +946,28 @@ Fp8Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated, bool native) {
         p.slabs = gated ? static_cast<size_t>(4 * M * N) : p.splits > 1 ? static_cast<size_t>(slab) * p.splits : 0;   // gated: act(g) * u
         return p;
     }
+    const int products = gated ? 2 : 1;
+    const double weights = static_cast<double>(products * N * K) * (K % kTileK ? 1.3 : 1.0);   // (rows that start inside a cache line)
     double best = 1e30;
     for (int i = 0; i < 4; ++i) {
-        const double us = big_us(i, M, N, nt, gated, native);
+        const double us = big_us(i, M, N, nt, weights, gated, native);
         if (us < best) {
             best = us;
             p.big = 256 - 64 * i;
         }
     }
-    const int products = gated ? 2 : 1;
-    const double stream = static_cast<double>(products * N * K) / 4.5e6;   // us, at 4.5 TB/s
     constexpr int64_t kMostSlabs = int64_t{1} << 28;
     static constexpr int kSlices[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
-    for (const TileFit& t : kTiles) {
+    for (const Tile& t : kTiles) {
         const int64_t tiles = ceil_div(M, t.rows) * ceil_div(N, t.rows == 128 ? 128 : 64) * products;
         for (const int s : kSlices) {
             if (s > 1 && (s > nt / 2 || tiles * s > 6 * kCus)) break;
             const int64_t kt = ceil_div(nt, s), slices = nt > 0 ? ceil_div(nt, kt) : 1;
-            double us = tile_us(t, tiles * slices, kt, native);
-            if (us < stream) us = stream;
+            double us = tile_us(t, tiles * slices, kt, weights, native);
             if (slices > 1 || gated) {
                 const int64_t bytes = products * slices * slab;
                 if (bytes > kMostSlabs) break;
-                us += 4.0 + static_cast<double>(bytes) / 3.0e6;   // written and read
+                us += 4.0 + static_cast<double>(bytes) / 3.0e6;   // the second launch (as much of the host); slabs written and read
             }
             if (us >= best) continue;
             best = us;
