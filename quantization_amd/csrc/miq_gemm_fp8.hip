@@ -486,28 +486,30 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
     const int n0 = tn * kCols;
     const int mrows = static_cast<int>(g.M - m0 < kRows ? g.M - m0 : kRows), nrows = g.N - n0 < kCols ? g.N - n0 : kCols;
 
-    // Staging: a wave-instruction moves 8 rows x 128 B; wave v moves rows v * 8 + 64 i, i = 0 .. 3, of each operand.  K-tile
-    // and row group advance in the descriptor (scalar registers); a lane's offset stays.  Rows past the matrix lie past the
-    // descriptor's end and read as zeros.
+    // Staging: a wave-instruction moves 8 rows x 128 B; wave v moves rows v * 8 + 64 i, i = 0 .. 3, of each operand.  K-tile and
+    // row group are in the lane's offset; rows past the matrix lie past the descriptor's end and read as zeros.  The operand is
+    // picked by value, without a branch: a branch would leave the compiler unsure how many requests are younger than a scale's,
+    // and it would wait for all of them before the scale's use.
     const int srow = wave * 8 + (lane >> 3);
     const int cbyte = ((lane & 7) ^ ((srow >> 1) & 7)) * kChunk;
-    const uint32_t off0 = static_cast<uint32_t>(srow) * static_cast<uint32_t>(g.K) + cbyte;
-    // An operand's rows 0-127 and 128-255: first row, and how many exist (may be negative).
+    const uint32_t off0 = static_cast<uint32_t>(srow) * static_cast<uint32_t>(g.K) + cbyte, rows64 = 64u * static_cast<uint32_t>(g.K);
     const uint8_t* const x0 = g.x + m0 * g.K;
     const uint8_t* const w0 = g.w[0] + static_cast<int64_t>(n0) * g.K;
-    const uint8_t* const w128 = GATED ? g.w[1] + static_cast<int64_t>(n0) * g.K : w0 + 128ll * g.K;
-    const int w128_count = GATED ? nrows : nrows - 128;
+    const uint8_t* const w1 = g.w[GATED ? 1 : 0] + static_cast<int64_t>(n0) * g.K;
+    const uint32_t xbytes = static_cast<uint32_t>(mrows) * static_cast<uint32_t>(g.K), wbytes = static_cast<uint32_t>(nrows) * static_cast<uint32_t>(g.K);
     // K-tile kt of the rows of w (else of x) to the 32 KiB at byte `slot` of LDS
     auto stage = [&](bool of_w, int kt, int slot) {
         const int k = kt * kTileK;
-        const uint32_t off = k + cbyte < g.K ? off0 : kOob;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint8_t* rows = i < 2 ? (of_w ? w0 : x0) : (of_w ? w128 : x0 + 128ll * g.K);
-            const int count = i < 2 ? (of_w ? nrows : mrows) : (of_w ? w128_count : mrows - 128);
-            const int left = (count - (i & 1) * 64) * g.K - k;   // bytes from the piece's first row to the end
-            dma16(make_rsrc(rows + (i & 1) * 64ll * g.K + k, left > 0 ? left : 0), smem + slot + (wave + 8 * i) * (8 * kTileK), off);
-        }
+        const uint32_t off = k + cbyte < g.K ? off0 + k : kOob;
+        const uint32_t bytes = of_w ? wbytes : xbytes;
+        const uint8_t* const first = of_w ? w0 : x0;
+        const uint8_t* const second = GATED && of_w ? w1 : first;   // of rows 128 .. 255: the other weight's, or 128 rows on
+        const uint32_t on = GATED && of_w ? 0 : 2 * rows64;
+        char* const to = smem + slot + wave * (8 * kTileK);
+        dma16(make_rsrc(first, bytes), to, off);
+        dma16(make_rsrc(first, bytes), to + 64 * kTileK, off + rows64);
+        dma16(make_rsrc(second, bytes), to + 128 * kTileK, off + on);
+        dma16(make_rsrc(second, bytes), to + 192 * kTileK, off + on + rows64);
     };
     auto x_slot = [](int slot) { return slot * kSlot; };
     auto w_slot = [](int kt) { return (3 + (kt & 1)) * kSlot; };
@@ -597,18 +599,21 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    // Every request of the four youngest pieces' phase or later may be in flight, everything older has landed; and this wave's
-    // LDS reads have returned (the slots that they read are written after the barrier).
-    auto wait_all_but_one_slot = [] { asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory"); };
+    // The youngest four pieces may be in flight (`with_scale`: and a row scale requested beside them), everything older has
+    // landed; and this wave's LDS reads have returned (the slots that they read are written after the barrier).
+    auto wait_all_but_one_slot = [](auto with_scale) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(with_scale.value ? 5 : 4) : "memory");
+    };
+    using One = std::integral_constant<bool, (RF > 4)>;   // row scales of a second half of the wave's rows
     auto wait_reads = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
     if (nt > 0) {
-        uint32_t sv0 = row_scales(0, 0), sv1 = row_scales(0, 1);
+        uint32_t sv0 = row_scales(0, 0), sv1 = RF > 4 ? row_scales(0, 1) : 0;
         keep_order();
         stage(false, 0, x_slot(0));
         stage(true, 0, w_slot(0));
         keep_order();
         stage(false, 1, x_slot(1));
-        wait_all_but_one_slot();   // x(0), w(0)
+        wait_all_but_one_slot(std::false_type{});   // x(0), w(0)
         barrier();
         int group = wm;
         if (group == 1) {
@@ -623,25 +628,35 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
             slot = slot == 2 ? 0 : slot + 1;
             const float sw0 = ws0[t], sw1 = GATED ? ws1[t] : sw0;
             // phase A
-            stage(group == 0, group ? t + 2 : t + 1, group ? x_slot(ahead) : w_slot(t + 1));
-            xf[0] = operand<NATIVE>(read(xt, 0));
+            Codes codes[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) wf[j] = operand<NATIVE>(read(wt, w_row(j)));
+            for (int j = 0; j < 4; ++j) codes[j] = read(wt, w_row(j));
+            raw = read(xt, 0);
+            keep_order();
+            stage(group == 0, group ? t + 2 : t + 1, group ? x_slot(ahead) : w_slot(t + 1));   // (while the reads are on their way)
+            keep_order();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) wf[j] = operand<NATIVE>(codes[j]);
+            xf[0] = operand<NATIVE>(raw);
             if constexpr (!NATIVE) raw = read(xt, 16);
             static_for<0, AS>([&](auto i) { rows_step(i, xt, sv0, sw0, sw1); });
-            if (group) wait_all_but_one_slot();   // x(t + 1), w(t + 1); x(t + 2) stays in flight
+            if (group) wait_all_but_one_slot(std::false_type{});   // x(t + 1), w(t + 1); x(t + 2) stays in flight
             else wait_reads();
             barrier();
-            // phase B: the next scales are requested ahead of the pieces, so that the wait behind these covers them
+            // phase B: the next scales, each into the register that it replaces: the first half's is free, the second half's
+            // after row fragment 4 (a copy at the loop's end would wait for the request, and for all pieces before it)
             const int tn1 = t + 1 < nt ? t + 1 : t;
             sv0 = row_scales(tn1, 0);
-            const uint32_t sv1_next = row_scales(tn1, 1);
             keep_order();
             stage(group != 0, t + 2, group ? w_slot(t + 2) : x_slot(ahead));
-            static_for<AS, RF>([&](auto i) { rows_step(i, xt, sv1, sw0, sw1); });
-            sv1 = sv1_next;
+            keep_order();
+            constexpr int kLast = RF > 4 ? 5 : RF;   // (the row fragments behind it have their scales already)
+            static_for<AS, kLast>([&](auto i) { rows_step(i, xt, sv1, sw0, sw1); });
+            if constexpr (RF > 4) sv1 = row_scales(tn1, 1);
+            keep_order();
+            static_for<kLast, RF>([&](auto i) { rows_step(i, xt, sv1, sw0, sw1); });
             if (group) wait_reads();
-            else wait_all_but_one_slot();
+            else wait_all_but_one_slot(One{});
             barrier();
         }
         if (wm == 0) barrier();   // every wave executes the same number of barriers
