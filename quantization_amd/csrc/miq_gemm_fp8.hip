@@ -137,22 +137,6 @@ __device__ __forceinline__ void store4(void* out, int64_t i, int n, bool vec, v4
 // Memory requests before this stay before it, those after it after: the counted waits below depend on the order of issue.
 __device__ __forceinline__ void keep_order() { asm volatile("" ::: "memory"); }
 
-// Fills one LDS tile with 16-byte LDS-DMA: K-tile kt of the ROWS rows at `rows`, `nrows` of which exist (the others, and
-// columns past K, read as zeros).
-template <int ROWS, int NWAVES>
-__device__ __forceinline__ void stage_rows(const uint8_t* rows, int nrows, int K, int kt, char* tile, int wave, int lane) {
-    constexpr int kPieces = ROWS / 8, kIters = (kPieces + NWAVES - 1) / NWAVES;
-    const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(rows, static_cast<uint32_t>(nrows) * static_cast<uint32_t>(K));
-#pragma unroll
-    for (int i = 0; i < kIters; ++i) {
-        const int piece = wave + i * NWAVES;   // wave-uniform
-        if (kPieces % NWAVES != 0 && piece >= kPieces) break;
-        const int r = piece * 8 + (lane >> 3);
-        const int k = kt * kTileK + ((lane & 7) ^ ((r >> 1) & 7)) * kChunk;
-        dma16(rsrc, tile + piece * (8 * kTileK), r < nrows && k < K ? static_cast<uint32_t>(r) * static_cast<uint32_t>(K) + k : kOob);
-    }
-}
-
 // Rows of K bytes -> rows of `pitch` bytes (K rounded up to 16), zeros past K: one thread a 16-byte piece, up to three
 // matrices in one launch.
 struct PadArgs {
@@ -205,7 +189,8 @@ __device__ __forceinline__ void wave_lds_order() {
 constexpr int tile_stage_bytes(int bm, int bn, int waves) { return (bm + bn) * kTileK + waves * ((bm + 63) / 64) * 256; }
 
 template <int BM, int BN, int WAVES_M, int WAVES_N, int STAGES, int OUT, bool NATIVE>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(Fp8Args g) {
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gemm_fp8_tile_kernel(Fp8Args g) {   // (2: at most 256 registers, and
+    // no matrix results in accumulation registers, which the vector unit would have to fetch from there one by one)
     constexpr int NWAVES = WAVES_M * WAVES_N;
     constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, FM = WM / 16, FN = WN / 16;
     constexpr int kRowBytes = (BM + BN) * kTileK, kScaleLoads = (BM + 63) / 64;
@@ -223,8 +208,14 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
     const int64_t m0 = static_cast<int64_t>(tm) * BM;
     const int n0 = tn * BN;
     const int mrows = static_cast<int>(g.M - m0 < BM ? g.M - m0 : BM), nrows = g.N - n0 < BN ? g.N - n0 : BN;
-    const uint8_t* xrows = g.x + m0 * g.K;
-    const uint8_t* wrows = g.w[which] + static_cast<int64_t>(n0) * g.K;
+    // Staging: a wave-instruction moves 8 rows x 128 B; wave v moves rows v * 8 + 8 NWAVES i.  Rows past the matrix lie past the
+    // descriptor's end and read as zeros.
+    const int srow = wave * 8 + (lane >> 3), cbyte = ((lane & 7) ^ ((srow >> 1) & 7)) * kChunk;
+    const uint32_t off0 = static_cast<uint32_t>(srow) * static_cast<uint32_t>(g.K) + cbyte;
+    const uint32_t piece_rows = 8u * NWAVES * static_cast<uint32_t>(g.K);
+    const __amdgpu_buffer_rsrc_t rx = make_rsrc(g.x + m0 * g.K, static_cast<uint32_t>(mrows) * static_cast<uint32_t>(g.K));
+    const __amdgpu_buffer_rsrc_t rw =
+        make_rsrc(g.w[which] + static_cast<int64_t>(n0) * g.K, static_cast<uint32_t>(nrows) * static_cast<uint32_t>(g.K));
     using scalar_floats = const __attribute__((address_space(4))) float*;   // (read through the scalar unit)
     const scalar_floats wscale = (scalar_floats)(g.ws[which] + static_cast<int64_t>(n0 / 128) * g.kblocks);
 
@@ -239,11 +230,17 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
     const int lo0 = frag_lane_offset(lane, 0), lo1 = frag_lane_offset(lane, 1);
     // A stage of LDS: BM + BN rows of a K-tile, and for each wave a copy of the rows' scales (fetched by LDS-DMA like the rows:
     // a scale loaded into a register would be waited for together with the younger rows' requests).
+    const float* xs_at = g.xs + static_cast<int64_t>(kt0) * g.M + m0;   // of the K-tile that stage() is called for next
     auto stage = [&](char* buf, int kt) {   // (a K-tile past the slice is requested out of range: zeros, no memory traffic)
-        const int k = kt < kt1 ? kt : g.kblocks;
-        stage_rows<BM, NWAVES>(xrows, mrows, g.K, k, buf, wave, lane);
-        stage_rows<BN, NWAVES>(wrows, nrows, g.K, k, buf + BM * kTileK, wave, lane);
-        const __amdgpu_buffer_rsrc_t rs = make_rsrc(g.xs + static_cast<int64_t>(kt < kt1 ? kt : kt0) * g.M + m0, kt < kt1 ? static_cast<uint32_t>(mrows) * 4 : 0);
+        const int k = (kt < kt1 ? kt : g.kblocks) * kTileK;
+        const uint32_t off = k + cbyte < g.K ? off0 + k : kOob;
+        char* const to = buf + wave * (8 * kTileK);
+#pragma unroll
+        for (int i = 0; i < BM / 8 / NWAVES; ++i) dma16(rx, to + i * (8 * NWAVES * kTileK), off + i * piece_rows);
+#pragma unroll
+        for (int i = 0; i < BN / 8 / NWAVES; ++i) dma16(rw, to + BM * kTileK + i * (8 * NWAVES * kTileK), off + i * piece_rows);
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(xs_at, kt < kt1 ? static_cast<uint32_t>(mrows) * 4 : 0);
+        xs_at += g.M;
 #pragma unroll
         for (int i = 0; i < kScaleLoads; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(buf + kRowBytes + (wave * kScaleLoads + i) * 256), 4,
@@ -285,15 +282,15 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gemm_fp8_tile_kernel(F
                 stage(smem + t * STAGE, kt0 + t);
                 keep_order();
             }
-            int slot = 0, fill = STAGES - 1;
+            int slot = 0, fill = (STAGES - 1) * STAGE;
             for (int kt = kt0; kt < kt1; ++kt) {
                 asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kKeep) : "memory");
                 __builtin_amdgcn_s_barrier();   // K-tile kt is there for every wave; every wave has read kt - 1
                 keep_order();
-                stage(smem + fill * STAGE, kt + STAGES - 1);
-                multiply(smem + slot * STAGE, kt);
-                slot = slot + 1 == STAGES ? 0 : slot + 1;
-                fill = fill + 1 == STAGES ? 0 : fill + 1;
+                stage(smem + fill, kt + STAGES - 1);
+                multiply(smem + slot, kt);
+                fill = slot;   // (the slot that was just read takes the K-tile STAGES - 1 on)
+                slot = slot == (STAGES - 1) * STAGE ? 0 : slot + STAGE;
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
@@ -916,8 +913,8 @@ double overlapped_us(double work, double weights, double rate) {
 }
 // One workgroup a CU: as many rounds as the tiles need, each a time a K-tile and a prologue and epilogue.
 double big_us(int i, int64_t M, int64_t N, int64_t nt, double weights, bool gated, bool native) {
-    static constexpr BigFit kFit[2][4] = {{{3.05, 12.9}, {2.46, 10.7}, {1.94, 8.5}, {1.50, 5.0}},   // bf16 form: 256 to 64 rows
-                                          {{1.72, 9.0}, {1.34, 9.1}, {1.12, 6.0}, {1.03, 3.9}}};    // 8-bit form
+    static constexpr BigFit kFit[2][4] = {{{2.89, 13.0}, {2.26, 11.2}, {1.70, 8.8}, {1.23, 5.3}},   // bf16 form: 256 to 64 rows
+                                          {{1.61, 10.0}, {1.19, 9.6}, {1.0, 6.2}, {0.91, 4.2}}};    // 8-bit form
     const BigFit& f = kFit[native][i];
     const int64_t tiles = ceil_div(M, 256 - 64 * i) * ceil_div(N, gated ? 128 : 256);
     return 1.0 + overlapped_us(static_cast<double>(ceil_div(tiles, kCus)) * (f.k_tile * static_cast<double>(nt) + f.round), weights, 2.8);
