@@ -898,10 +898,10 @@ constexpr int64_t kCus = 256;
 // Above 16 rows the large kernel and the tile kernel, the latter with tiles of three heights and K in any number of slices, can
 // all run a product: the one with the smallest estimate does.  The estimates' constants are us, fitted to the times of every
 // variant on 227 shapes from 17x64x128 to 8192x28672x28672 (the estimates are within 12% of the times, the choice within 3% of
-// the best variant's time on average).  E.g. 512x2048x2048 bf16: large kernel 19.2 (64 rows), 128-row tiles 16.6, 64 9.1, 64 in
-// two slices 14.4; 254x354x2560 bf16 23.5, 128-row tiles in two slices 13.6, 32-row tiles whole 8.5, in four slices 7.5; gated
-// 2785x669x10032 163 (128 rows), 128-row tiles in two slices 123, in four 113; gated 2773x5456x224 34.6 (256 rows), 128-row tiles
-// 56; fp32 1000x10001x4000 91 (192 rows), 107 (256), 128-row tiles 100.
+// the best variant's time on average).  E.g. 512x2048x2048 bf16: 64-row tiles 9.0, in two slices 14.8, 128-row tiles 17.3, the
+// large kernel 16.3 (64 rows); 254x354x2560 bf16: 32-row tiles in four slices 7.7, 64-row tiles whole 9.0, the large kernel 19.4;
+// gated 2785x669x10032: 128-row tiles in four slices 112, in two 122, the large kernel 143 (128 rows); gated 2773x5456x224: the
+// large kernel 34 (256 rows), 128-row tiles 57; fp32 1000x10001x4000: the large kernel 84 (192 rows), 101 (256), 128-row tiles 97.
 struct BigFit {
     double k_tile, round;
 };
@@ -913,11 +913,11 @@ double overlapped_us(double work, double weights, double rate) {
 }
 // One workgroup a CU: as many rounds as the tiles need, each a time a K-tile and a prologue and epilogue.
 double big_us(int i, int64_t M, int64_t N, int64_t nt, double weights, bool gated, bool native) {
-    static constexpr BigFit kFit[2][4] = {{{2.89, 13.0}, {2.26, 11.2}, {1.70, 8.8}, {1.23, 5.3}},   // bf16 form: 256 to 64 rows
-                                          {{1.61, 10.0}, {1.19, 9.6}, {1.0, 6.2}, {0.91, 4.2}}};    // 8-bit form
+    static constexpr BigFit kFit[2][4] = {{{2.88, 12.9}, {2.25, 11.2}, {1.68, 8.9}, {1.22, 5.4}},   // bf16 form: 256 to 64 rows
+                                          {{1.58, 10.0}, {1.16, 9.5}, {0.98, 6.2}, {0.91, 4.2}}};   // 8-bit form
     const BigFit& f = kFit[native][i];
     const int64_t tiles = ceil_div(M, 256 - 64 * i) * ceil_div(N, gated ? 128 : 256);
-    return 1.0 + overlapped_us(static_cast<double>(ceil_div(tiles, kCus)) * (f.k_tile * static_cast<double>(nt) + f.round), weights, 2.8);
+    return 3.0 + overlapped_us(static_cast<double>(ceil_div(tiles, kCus)) * (f.k_tile * static_cast<double>(nt) + f.round), weights, 2.8);
 }
 // `groups` workgroups of `kt` K-tiles each, `resident` on a CU.  A workgroup alone on its CU takes `alone` a K-tile (a fetch and
 // its own matrix work), a full CU `full` for each workgroup's; `stream` is the rate of the weights' stream, bytes a ps.
@@ -928,9 +928,9 @@ struct Tile {
     int rows, resident;
     TileFit fit[2];   // bf16 form, 8-bit form
 };
-constexpr Tile kTiles[3] = {{32, 4, {{3.85, 0.34, 0.24, 5.25}, {3.2, 0.26, 0.20, 5.25}}},
-                            {64, 3, {{4.1, 0.445, 0.345, 5.25}, {3.5, 0.34, 0.283, 5.25}}},
-                            {128, 2, {{5.7, 1.08, 0.927, 4.45}, {4.4, 0.95, 0.69, 4.0}}}};
+constexpr Tile kTiles[3] = {{32, 4, {{4.1, 0.30, 0.228, 6.0}, {3.5, 0.223, 0.198, 5.9}}},
+                            {64, 3, {{4.5, 0.414, 0.321, 6.0}, {3.7, 0.29, 0.285, 5.9}}},
+                            {128, 2, {{5.9, 1.12, 0.916, 5.2}, {4.2, 1.06, 0.672, 4.25}}}};
 double tile_us(const Tile& t, int64_t groups, int64_t kt, double weights, bool native) {
     const TileFit& f = t.fit[native];
     const int64_t deep = ceil_div(groups, kCus);   // workgroups of the busiest CU
@@ -979,7 +979,7 @@ Fp8Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated, bool native) {
             if (slices > 1 || gated) {
                 const int64_t bytes = products * slices * slab;
                 if (bytes > kMostSlabs) break;
-                us += 4.0 + static_cast<double>(bytes) / 3.0e6;   // the second launch (as much of the host); slabs written and read
+                us += 3.5 + 0.15 * static_cast<double>(slices) + static_cast<double>(bytes) / 3.3e6;   // second launch; slabs written, read
             }
             if (us >= best) continue;
             best = us;
@@ -1010,12 +1010,19 @@ int launch_tile(Fp8Args g, int splits, int products, hipStream_t st) {
     return check_launch("gemm_fp8_tile_kernel");
 }
 // NATIVE16: the products of a 16-bit output (the slabs' sums included) may use the 8-bit instruction.  Stages and waves as
-// measured: a ring of three K-tiles fits three workgroups a CU, one of four two (48x14336x4096 bf16 17.5 us against 19.3); 128 x
-// 128 tiles as eight waves of 32 x 64 (256x4096x14336 bf16 32.4 us, as four of 64 x 64 34.7, with a ring of three 49.7).
+// measured: a ring of three K-tiles fits three workgroups a CU, one of four two (77x14336x4096 bf16 16.9 us against 17.2), one of
+// two waits for each fetch (21.8); 64 x 64 tiles as four waves of 32 x 32 (as two of 32 x 64 21.0); 128 x 128 tiles as eight
+// waves of 32 x 64 (256x4096x14336 bf16 31.9 us, as four of 64 x 64 32.7, with a ring of three 38.9).  A 64 x 64 tile that has
+// its CU to itself goes to eight waves on the 8-bit instruction: nothing else covers a wave's wait (128x8192x8192 bf16 21.6 us,
+// four waves 25.9; two workgroups a CU: 512x4096x4096 17.7 and 17.3; widening, eight waves lose: 427x5073x3712 36.2 and 30.0).
 template <int OUT, bool NATIVE16>
 int launch_tiles(const Fp8Plan& p, const Fp8Args& g, int products, hipStream_t st) {
     if (p.bm == 32) return launch_tile<32, 64, 2, 2, 3, OUT, NATIVE16>(g, p.splits, products, st);
-    if (p.bm == 64) return launch_tile<64, 64, 2, 2, 3, OUT, NATIVE16>(g, p.splits, products, st);
+    if (p.bm == 64) {
+        if constexpr (NATIVE16)
+            if (ceil_div(g.M, 64) * ceil_div(g.N, 64) * p.splits * products <= kCus) return launch_tile<64, 64, 4, 2, 3, OUT, NATIVE16>(g, p.splits, products, st);
+        return launch_tile<64, 64, 2, 2, 3, OUT, NATIVE16>(g, p.splits, products, st);
+    }
     return launch_tile<128, 128, 4, 2, 2, OUT, NATIVE16>(g, p.splits, products, st);
 }
 
