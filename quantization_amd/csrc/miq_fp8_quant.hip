@@ -10,7 +10,8 @@ namespace {
 using namespace miq;
 
 // ---- activations: 1 x 128 ------------------------------------------------------------------------------------------
-// A workgroup of 16 sixteen-lane groups takes ROWS rows x (16 / ROWS) * kQuantPasses blocks.
+// A workgroup of 16 sixteen-lane groups takes ROWS rows x (16 / ROWS) * kQuantPasses blocks.  Bound by HBM: 2048x14336 bf16
+// 16.0-16.5 us (5.4 TB/s read and written; a copy 4.9), fp32 28.0 (5.2); few rows by the launch, 2.5 us up to 64x14336.
 template <int DT, bool VEC, int ROWS, int kQuantPasses>
 __global__ __launch_bounds__(256) void quantize_blocks_kernel(const void* __restrict__ x, int64_t M, int64_t K, int64_t kblocks,
                                                               int64_t col_groups, uint8_t* __restrict__ q,
@@ -38,7 +39,8 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(const void* __rest
 }
 
 // ---- weights: 128 x 128 --------------------------------------------------------------------------------------------
-// One workgroup a block: a thread holds eight columns of eight rows (64 values) in registers.
+// One workgroup a block: a thread holds eight columns of eight rows (64 values) in registers, so that the weight is read once.
+// Bound by HBM: 14336x4096 fp32 50 us (5.9 TB/s), bf16 32.8 (5.4); rows that start anywhere (14336x4095 fp32) 86.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void quantize_weight_kernel(const void* __restrict__ w, int64_t N, int64_t K, int64_t kblocks,
                                                               uint8_t* __restrict__ q, float* __restrict__ scale) {
@@ -101,7 +103,8 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const void* __rest
 // ---- root-mean-square norm -----------------------------------------------------------------------------------------
 // h = x + residual (rounded to the type it is stored in, so that the norm is the norm of the stored row), y = (h / rms) * g,
 // then y in blocks as above.  TPR threads a row; a row of at most TPR * 8 * VPT columns stays in registers between the sum
-// of squares and the codes (VPT > 0); a longer one is read twice (VPT = 0).
+// of squares and the codes (VPT > 0); a longer one is read twice (VPT = 0).  Bound by HBM: 8192x8192 bf16 with a residual 82.5 us
+// (5.7 TB/s), 8192x4096 44.3 (5.3), 1024x40000, read twice, 81.6 (3.5 TB/s of 7 bytes an element); one row 3.2 us, a launch.
 template <int DT>
 __device__ __forceinline__ float round_to(float v) {
     if constexpr (DT == MIQ_BF16) return static_cast<float>(static_cast<__bf16>(v));
@@ -113,13 +116,11 @@ template <int DT, bool VEC>
 __device__ __forceinline__ void store8(void* base, int64_t index, int n, const float (&f)[8]) {
     if constexpr (DT == MIQ_F32) {
         float* p = static_cast<float*>(base) + index;
-        if constexpr (VEC) {
-            if (n > 0) {
-                typedef float f32x4 __attribute__((ext_vector_type(4)));
-                reinterpret_cast<f32x4*>(p)[0] = f32x4{f[0], f[1], f[2], f[3]};
-                reinterpret_cast<f32x4*>(p)[1] = f32x4{f[4], f[5], f[6], f[7]};
-            }
-        } else {
+        if (n == 8) {
+            auto bits = [&](int i) { return __float_as_uint(f[i]); };
+            *reinterpret_cast<u32x4_any*>(p) = u32x4{bits(0), bits(1), bits(2), bits(3)};
+            *reinterpret_cast<u32x4_any*>(p + 4) = u32x4{bits(4), bits(5), bits(6), bits(7)};
+        } else if (!VEC) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (i < n) p[i] = f[i];
@@ -132,14 +133,12 @@ __device__ __forceinline__ void store8(void* base, int64_t index, int n, const f
             if constexpr (DT == MIQ_BF16) h[i] = __builtin_bit_cast(uint16_t, static_cast<__bf16>(f[i]));
             else h[i] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(f[i]));
         }
-        if constexpr (VEC) {
-            if (n > 0) {
-                u32x4 v;
+        if (n == 8) {
+            u32x4 v;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = h[2 * i] | (static_cast<uint32_t>(h[2 * i + 1]) << 16);
-                __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(p));   // (8192 x 8192 with a residual: 95 us, 101 cached)
-            }
-        } else {
+            for (int i = 0; i < 4; ++i) v[i] = h[2 * i] | (static_cast<uint32_t>(h[2 * i + 1]) << 16);
+            __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(p));   // (8192 x 8192 with a residual: 95 us, 101 cached)
+        } else if (!VEC) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (i < n) p[i] = h[i];
@@ -266,8 +265,9 @@ extern "C" int miq_quantize_blocks_fp8(const void* x, int x_dtype, int64_t M, in
     MIQ_REQUIRE(aligned(x, elem_size(x_dtype)) && aligned(scale, 4), MIQ_EALIGN, "miq_quantize_blocks_fp8: misaligned pointer");
     const bool vec = K % 8 == 0 && aligned(x, 16) && aligned(q, 8);
     const int64_t kblocks = ceil_div(K, kBlockK);
-    // Sixteen rows of a block at a time where there are as many, so that their scales leave as one line; four blocks a thread
-    // in flight, or one where that would leave CUs idle (a few rows: the launch is all latency).
+    // Sixteen rows of a block at a time where there are as many, so that their scales leave as one line (2048x14336 bf16 16.5 us,
+    // rows one by one 18.2; fewer rows are a launch either way); four blocks a thread in flight (16.4 us; one: 17.3), or one
+    // where four would leave CUs idle (64x4096 2.5 us, four 3.3; 256x4096 2.7 and 3.7; 512x14336 5.9 both).
     const bool tall = M >= 16, few = ceil_div(M, tall ? 16 : 1) * ceil_div(kblocks, tall ? 4 : 64) < 256;
     const int64_t col_groups = ceil_div(kblocks, (tall ? 1 : 16) * (few ? 1 : 4));
     const int64_t grid = (tall ? ceil_div(M, 16) : M) * col_groups;
@@ -334,7 +334,8 @@ extern "C" int miq_rms_norm_fp8(const void* x, const void* residual, const void*
             constexpr bool V = decltype(v)::value;
             const unsigned grid = static_cast<unsigned>(M);
             // Two vectors a thread where a row has as many threads (8192 x 8192 bf16 with a residual: 83 us as 512 threads of
-            // two, 90 as 256 of four, 109 as 1024 of one); four keep rows of up to 32768 columns in registers.
+            // two, 90 as 256 of four, 109 as 1024 of one; 8192x4096 44 as 256 of two, 49 as 512; 8192x2048 23.6 as 256 of one,
+            // 36 as 512); four keep rows of up to 32768 columns in registers (2048x28672 88 us, read twice 116).
             if (cols <= 256 * 8) rms_norm_kernel<DT, V, 256, 1><<<grid, 256, 0, as_stream(stream)>>>(a);
             else if (cols <= 256 * 16) rms_norm_kernel<DT, V, 256, 2><<<grid, 256, 0, as_stream(stream)>>>(a);
             else if (cols <= 512 * 16) rms_norm_kernel<DT, V, 512, 2><<<grid, 512, 0, as_stream(stream)>>>(a);

@@ -12,7 +12,13 @@
 // of it (measured: 2^16 + 2^2 gives 2^16 where 2^16 + 2^3 is right; across groups of eight it keeps 24 bits).  On layers'
 // operands that is 3e-5 of the result, a hundred times an fp32 sum's error.  v_mfma_f32_16x16x32_bf16 keeps 24 bits
 // throughout (1e-8 on the same operands), and e4m3 widens to bf16 exactly (v_cvt_scalef32_pk_bf16_fp8, two codes an
-// instruction), at half the rate.
+// instruction), at half the rate.  So 16-bit outputs, whose own rounding is 60 to 100 times coarser, take the 8-bit
+// instruction; fp32 outputs, the gated product (its scales are fp32) and products of at most 16 rows (which the weight's
+// stream bounds in either form) widen.
+//
+// What a block's scale costs: an accumulator is written by the vector unit once a K-tile, one fused multiply-add an output,
+// beside the matrix instructions; a product with one scale for a whole tensor has none of that.  The 16 x 16 instructions
+// leave it room: a SIMD issues two vector instructions in the time of one 16x16x32 bf16 instruction without slowing it.
 #include <cmath>
 
 #include "miq_fp8.h"
@@ -186,6 +192,10 @@ __device__ __forceinline__ void wave_lds_order() {
 // a fetch; STAGES > 2: a ring with STAGES - 1 K-tiles in flight and a counted wait, for the thin ones (a few rows against a
 // weight that streams from HBM), whose K-tile of matrix work is far shorter than a fetch.  Split-K: slice blockIdx.y sums its
 // K-tiles into an fp32 slab of its own; blockIdx.z picks the weight of a gated product.
+//
+// Bound by the weight's stream where there are few rows (77x14336x4096 bf16: 16.5 us, 3.7 TB/s of weight; 24x14336x4096 gated:
+// 28 us with the join, 4.2 TB/s), by its LDS reads and vector work above: a 64 x 64 tile reads 3 bytes of LDS for each byte it
+// fetches (1024x4096x4096 bf16 1.0 PFLOP/s with 64-row tiles, 1.2 with 128-row ones; fp32 427x5073x3712 30 us, 0.54).
 constexpr int tile_stage_bytes(int bm, int bn, int waves) { return (bm + bn) * kTileK + waves * ((bm + 63) / 64) * 256; }
 
 template <int BM, int BN, int WAVES_M, int WAVES_N, int STAGES, int OUT, bool NATIVE>
@@ -346,7 +356,9 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gemm_fp8_tile_kerne
 // loads the chunks that the instructions want from it.  A workgroup of kWaves waves owns GROUPS row groups; wave v sums
 // the K-tiles v, v + kWaves, ... (eight consecutive K-tiles are 1 KiB of a row), DEPTH of them in flight, and the partial
 // sums meet in LDS.  A gated product's groups are the gate's and the up projection's of the same columns: the workgroup
-// finishes act(g) * u in fp32, and the quantizer follows.
+// finishes act(g) * u in fp32, and the quantizer follows.  Bound by the weight's stream: 1x4096x14336 11.3 us (5.2 TB/s),
+// 1x28672x8192 44 us (5.3), the two weights of 1x14336x4096 26 us (4.5); K that is no multiple of 128, so that a row's K-tile
+// is two half lines, 3.3 (9x17784x10032 54 us).
 template <int GROUPS, int kWaves, int DEPTH, int OUT, int ACT>
 __global__ __launch_bounds__(64 * kWaves) void gemm_fp8_rows16_kernel(Fp8Args g) {
     constexpr bool GATED = ACT != kNoAct;
@@ -391,7 +403,8 @@ __global__ __launch_bounds__(64 * kWaves) void gemm_fp8_rows16_kernel(Fp8Args g)
             for (int j = 0; j < GROUPS; ++j) s.w[j].c[h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw[j], off, 0, 0));
             s.x.c[h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 0, 0));
         }
-        const __amdgpu_buffer_rsrc_t rs = make_rsrc(g.xs + static_cast<int64_t>(in ? kt : 0) * g.M, in ? static_cast<uint32_t>(g.M) * 4 : 0);
+        const __amdgpu_buffer_rsrc_t rs =
+            make_rsrc(g.xs + static_cast<int64_t>(in ? kt : 0) * g.M, in ? static_cast<uint32_t>(g.M) * 4 : 0);
         s.s = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, (lane & 15) * 4, 0, 0));
     };
 
@@ -440,15 +453,16 @@ struct GatedOut {
 };
 
 // ---- 256 x 256 outputs a workgroup: large products -----------------------------------------------------------------
-// Eight waves, 2 (rows) x 4 (columns), a wave owns 128 x 64 outputs: eight row fragments by four column fragments.
+// Eight waves, 2 (rows) x 4 (columns), a wave owns 128 x 64 outputs: eight row fragments by four column fragments (six, four
+// or two row fragments where 256 rows would leave CUs idle).
 //
 // Within a K-tile a wave keeps the four column fragments and walks its row fragments; the sums of an earlier fragment are
 // scaled into their accumulators behind the matrix instructions of a later one (two instructions later for the 8-bit form,
 // four chains later for the bf16 form), so that vector and matrix work overlap without waiting for each other.
 //
-// A K-tile is two phases, A (read and widen the column fragments, row fragments 0-3) and B (4-7), a barrier before each.
-// Waves 4-7, the second wave of every SIMD, run one phase behind waves 0-3: while one wave reads and widens its column
-// fragments the other keeps the matrix pipe busy.  With barrier 2t at the start of A(t) for waves 0-3:
+// A K-tile is two phases, A (read and widen the column fragments, the first half of the row fragments) and B (the others), a
+// barrier before each.  Waves 4-7, the second wave of every SIMD, run one phase behind waves 0-3: while one wave reads and
+// widens its column fragments the other keeps the matrix pipe busy.  With barrier 2t at the start of A(t) for waves 0-3:
 //     after barrier 2t + 1 the rows x(t - 1) are read by nobody any more:  DMA of x(t + 2) into their slot (three slots)
 //     after barrier 2t     the rows w(t - 2 + 1) likewise:                 DMA of w(t + 1) (two slots)
 //     before barrier 2t    every wave has waited for its share of x(t) and w(t), issued three and two phases earlier; the
@@ -458,6 +472,14 @@ struct GatedOut {
 //
 // GATED: the tile is 128 columns of both weights, a wave's column fragments 0, 1 the gate's and 2, 3 the up projection's
 // same 32 columns, so that a lane holds both factors of its outputs and the 128 columns are one block of the result.
+//
+// Measured: 8192x8192x8192 bf16 465-473 us (2.32-2.37 PFLOP/s; the library's product of the same size with one scale a tensor
+// 383), gated 4096x14336x4096 740-755 us (1.27-1.30; the library's bf16 product does 1.52), fp32 1000x10001x4000 82.5 us (0.97;
+// 240 tiles of 192 rows on 256 CUs).  Bound by the chip's power more than by any one pipe: the clock falls to 1.8 GHz (8-bit
+// form) and 2.0 GHz (bf16 form) of 2.4 while the matrix pipes are 56% and 53% and vector issue 47% and 57% of the cycles busy.
+// Without its LDS-DMA the 8-bit form took 385 us, without the scaling 445, without its reads of x 398; the bf16 form without
+// widening 581.  32 x 32 instructions, which leave the vector unit more issue slots, were no faster: their accumulators, sixteen
+// registers a piece, do not fit 256 rows beside the widened columns, and 192 rows took 825 us for 754.
 
 // f(FIRST), ..., f(END - 1) with the index a constant.
 template <int FIRST, int END, typename F>
@@ -493,7 +515,8 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
     const uint8_t* const x0 = g.x + m0 * g.K;
     const uint8_t* const w0 = g.w[0] + static_cast<int64_t>(n0) * g.K;
     const uint8_t* const w1 = g.w[GATED ? 1 : 0] + static_cast<int64_t>(n0) * g.K;
-    const uint32_t xbytes = static_cast<uint32_t>(mrows) * static_cast<uint32_t>(g.K), wbytes = static_cast<uint32_t>(nrows) * static_cast<uint32_t>(g.K);
+    const uint32_t xbytes = static_cast<uint32_t>(mrows) * static_cast<uint32_t>(g.K);
+    const uint32_t wbytes = static_cast<uint32_t>(nrows) * static_cast<uint32_t>(g.K);
     // K-tile kt of the rows of w (else of x) to the 32 KiB at byte `slot` of LDS
     auto stage = [&](bool of_w, int kt, int slot) {
         const int k = kt * kTileK;
@@ -804,6 +827,7 @@ __global__ __launch_bounds__(512) void gemm_fp8_256_kernel(Fp8Args g, GatedOut g
 }
 
 // ---- split products: the slabs' sums ---------------------------------------------------------------------------------
+// In the slices' order, whatever order they ended in.  Launch-bound: 2.8 to 3.7 us at these sizes, 0.15 us more a slice.
 // Eight consecutive sums of a row at `at`, over `splits` slabs of `size` floats, in order.
 __device__ __forceinline__ void sum_slabs(const float* __restrict__ slabs, int splits, int64_t size, int64_t at, float (&v)[8]) {
 #pragma unroll
@@ -841,7 +865,8 @@ __global__ __launch_bounds__(256) void splitk_sum_kernel(const float* __restrict
     }
 }
 
-// h = act(sum of the gate's slabs) * (sum of the up projection's), in blocks: sixteen lanes a block of one row.
+// h = act(sum of the gate's slabs) * (sum of the up projection's), in blocks: sixteen lanes a block of one row (48 rows of 14336:
+// 4.1 us for the 5.5 MB of two slabs, which come from the L2s and the Infinity Cache).
 template <int ACT>
 __global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict__ slabs, int splits, Fp8Args g, int nblocks,
                                                          uint8_t* __restrict__ q, float* __restrict__ scale) {
@@ -897,7 +922,7 @@ constexpr int64_t kCus = 256;
 
 // Above 16 rows the large kernel and the tile kernel, the latter with tiles of three heights and K in any number of slices, can
 // all run a product: the one with the smallest estimate does.  The estimates' constants are us, fitted to the times of every
-// variant on 227 shapes from 17x64x128 to 8192x28672x28672 (the estimates are within 12% of the times, the choice within 3% of
+// variant on 227 shapes, M 17 to 7701, N 65 to 28672, K 128 to 28672, 0.6 TFLOP at most (the estimates are within 12% of the times, the choice within 3% of
 // the best variant's time on average).  E.g. 512x2048x2048 bf16: 64-row tiles 9.0, in two slices 14.8, 128-row tiles 17.3, the
 // large kernel 16.3 (64 rows); 254x354x2560 bf16: 32-row tiles in four slices 7.7, 64-row tiles whole 9.0, the large kernel 19.4;
 // gated 2785x669x10032: 128-row tiles in four slices 112, in two 122, the large kernel 143 (128 rows); gated 2773x5456x224: the
@@ -1005,7 +1030,8 @@ int launch_tile(Fp8Args g, int splits, int products, hipStream_t st) {
     g.tiles_m = static_cast<int>(ceil_div(g.M, BM));
     g.tiles_n = static_cast<int>(ceil_div(g.N, BN));
     const dim3 grid(static_cast<unsigned>(g.tiles_m) * g.tiles_n, splits, products);
-    if (int rc = allow_lds(reinterpret_cast<const void*>(&gemm_fp8_tile_kernel<BM, BN, WAVES_M, WAVES_N, STAGES, OUT, NATIVE>), kLds)) return rc;
+    const void* fn = reinterpret_cast<const void*>(&gemm_fp8_tile_kernel<BM, BN, WAVES_M, WAVES_N, STAGES, OUT, NATIVE>);
+    if (int rc = allow_lds(fn, kLds)) return rc;
     gemm_fp8_tile_kernel<BM, BN, WAVES_M, WAVES_N, STAGES, OUT, NATIVE><<<grid, 64 * WAVES_M * WAVES_N, kLds, st>>>(g);
     return check_launch("gemm_fp8_tile_kernel");
 }
@@ -1019,8 +1045,9 @@ template <int OUT, bool NATIVE16>
 int launch_tiles(const Fp8Plan& p, const Fp8Args& g, int products, hipStream_t st) {
     if (p.bm == 32) return launch_tile<32, 64, 2, 2, 3, OUT, NATIVE16>(g, p.splits, products, st);
     if (p.bm == 64) {
+        const bool alone = ceil_div(g.M, 64) * ceil_div(g.N, 64) * p.splits * products <= kCus;
         if constexpr (NATIVE16)
-            if (ceil_div(g.M, 64) * ceil_div(g.N, 64) * p.splits * products <= kCus) return launch_tile<64, 64, 4, 2, 3, OUT, NATIVE16>(g, p.splits, products, st);
+            if (alone) return launch_tile<64, 64, 4, 2, 3, OUT, NATIVE16>(g, p.splits, products, st);
         return launch_tile<64, 64, 2, 2, 3, OUT, NATIVE16>(g, p.splits, products, st);
     }
     return launch_tile<128, 128, 4, 2, 2, OUT, NATIVE16>(g, p.splits, products, st);

@@ -415,10 +415,8 @@ def test_same_call_same_bits(m):
 
 @pytest.mark.parametrize("seed", range(8))
 def test_random_shapes(seed):
-    """Sizes spread over their logarithm; codes by the kernels' own quantizer (checked above, bit for bit), products on the
-    GPU in float64."""
+    """Sizes spread over their logarithm; the products on the GPU in float64."""
     import random
-    from quantization_amd import block_fp8 as F
     rng = random.Random(seed)
 
     def size(lo, hi):
@@ -428,28 +426,123 @@ def test_random_shapes(seed):
         step = rng.choice([1, 16, 128])
         k = max(step, size(1, 6000) // step * step)
         out, act = rng.choice(FLOATS), rng.choice(["silu", "gelu"])
-        xq, xs = F.quantize_blocks_fp8(rand(m, k, torch.float32, m).cuda())
-        w = [F.quantize_weight_fp8((rand(n, k, torch.float32, n + j) / math.sqrt(k)).cuda()) for j in range(2)]
-        bk, bn = torch.arange(k, device="cuda") // 128, torch.arange(n, device="cuda") // 128
-        x = xq.double() * xs.double().t()[:, bk]
-        ws = [q.double() * s.double()[bn][:, bk] for q, s in w]
-        ref, mag = x @ ws[0].t(), x.abs() @ ws[0].abs().t()
-        y = F.linear_fp8(xq, xs, *w[0], None, out)
-        err = R.product_error(mag, k) + dropped(out, m) * mag
-        tol = err + torch.finfo(out).eps / 2 * (ref.abs() + err) + torch.finfo(out).smallest_normal * torch.finfo(out).eps
-        fits = ref.abs() < torch.finfo(out).max * 0.99
-        off = (y.double() - ref).abs()
-        assert bool((off <= tol)[fits].all()), (m, n, k, out, float((off / tol)[fits].max()))
-        u, umag = x @ ws[1].t(), x.abs() @ ws[1].abs().t()
-        a = R.act(ref, act)
-        da = 1.13 * R.product_error(mag, k) + 8 * 2.0 ** -23 * ref.abs()
-        h = a * u
-        dh = da * (u.abs() + R.product_error(umag, k)) + a.abs() * R.product_error(umag, k) + 2.0 ** -23 * h.abs()
-        q, s = F.gated_linear_fp8(xq, xs, *w[0], *w[1], act)
-        try:
-            R.check_codes_of(q, s, h.cpu(), dh.cpu())
-        except AssertionError as e:
-            raise AssertionError(f"gated {m} x {n} x {k} {act}: {e}") from None
+        check_linear(m, n, k, out)
+        check_gated(m, n, k, act)
+
+
+def on_gpu(m, n, k, j):
+    """Codes and scales by the kernels' own quantizers (checked above, bit for bit), and the values that they stand for."""
+    from quantization_amd import block_fp8 as F
+    bk, bn = torch.arange(k, device="cuda") // 128, torch.arange(n, device="cuda") // 128
+    if m:
+        q, s = F.quantize_blocks_fp8(rand(m, k, torch.float32, m).cuda())
+        return (q, s), q.double() * s.double().t()[:, bk]
+    q, s = F.quantize_weight_fp8((rand(n, k, torch.float32, n + j) / math.sqrt(k)).cuda())
+    return (q, s), q.double() * s.double()[bn][:, bk]
+
+
+def check_linear(m, n, k, out, bias=False):
+    from quantization_amd import block_fp8 as F
+    (xq, xs), x = on_gpu(m, 0, k, 0)
+    w, wv = on_gpu(0, n, k, 0)
+    ref, mag = x @ wv.t(), x.abs() @ wv.abs().t()
+    err = R.product_error(mag, k) + dropped(out, m) * mag
+    b = None
+    if bias:
+        b = torch.randn(n, generator=torch.Generator().manual_seed(n)).cuda()
+        ref = ref + b.double()
+        err = err + 2.0 ** -24 * (ref.abs() + err)
+    y = F.linear_fp8(xq, xs, *w, b, out)
+    tol = err + torch.finfo(out).eps / 2 * (ref.abs() + err) + torch.finfo(out).smallest_normal * torch.finfo(out).eps
+    fits = ref.abs() < torch.finfo(out).max * 0.99
+    off = (y.double() - ref).abs()
+    assert bool((off <= tol)[fits].all()), (m, n, k, out, float((off / tol)[fits].max()))
+
+
+def check_gated(m, n, k, act):
+    from quantization_amd import block_fp8 as F
+    (xq, xs), x = on_gpu(m, 0, k, 0)
+    (w, wv), (w2, wv2) = on_gpu(0, n, k, 0), on_gpu(0, n, k, 1)
+    ref, mag = x @ wv.t(), x.abs() @ wv.abs().t()
+    u, umag = x @ wv2.t(), x.abs() @ wv2.abs().t()
+    a = R.act(ref, act)
+    da = 1.13 * R.product_error(mag, k) + 8 * 2.0 ** -23 * ref.abs()
+    h = a * u
+    dh = da * (u.abs() + R.product_error(umag, k)) + a.abs() * R.product_error(umag, k) + 2.0 ** -23 * h.abs()
+    q, s = F.gated_linear_fp8(xq, xs, *w, *w2, act)
+    try:
+        R.check_codes_of(q, s, h.cpu(), dh.cpu())
+    except AssertionError as e:
+        raise AssertionError(f"gated {m} x {n} x {k} {act}: {e}") from None
+
+
+# What a product of more than 16 rows can be run by: tiles of 32, 64 and 128 rows, whole and in slices of K, and the large
+# kernel with 64 to 256 rows; rows of outputs that are whole vectors and rows that are not.
+EVERY_16BIT = [(769, 7600, 64), (516, 11342, 64), (3294, 272, 4640), (2420, 385, 4448), (22, 64, 3184), (17, 75, 3344), (220, 7304, 64),
+               (3494, 404, 64), (4199, 88, 7793), (2765, 71, 8128), (33, 8696, 153), (33, 8222, 151), (1151, 72, 4400), (713, 68, 6992),
+               (425, 8256, 1984), (262, 10971, 2223), (6704, 600, 1680), (268, 13205, 1826), (3841, 2176, 1027), (385, 18395, 1040),
+               (651, 16856, 942), (783, 14542, 992)]
+EVERY_F32 = [(1932, 7904, 64), (2331, 6657, 64), (3294, 272, 4640), (2420, 385, 4448), (18, 72, 2192), (18, 69, 2448), (424, 5896, 64),
+             (262, 9341, 64), (1114, 72, 7104), (33, 2778, 5280), (7492, 808, 5120), (8297, 644, 5136), (942, 12760, 801),
+             (3252, 3773, 846), (5957, 2232, 1552), (579, 19833, 1584), (438, 9095, 10960)]
+EVERY_GATED = [(90, 5584, 64), (3754, 130, 64), (4182, 72, 4224), (4102, 74, 4480), (17, 72, 64), (19, 80, 432), (17, 66, 432), (880, 840, 272),
+               (4112, 132, 256), (2132, 72, 1114), (2330, 65, 1040), (1393, 352, 64), (2308, 784, 64), (193, 8764, 64), (8716, 400, 64),
+               (8294, 417, 64), (446, 11192, 64), (198, 16873, 64), (1000, 2000, 1000)]
+
+
+@pytest.mark.parametrize("m,n,k", EVERY_16BIT)
+def test_every_kernel_16_bit(m, n, k):
+    check_linear(m, n, k, torch.bfloat16 if n % 2 else torch.float16, bias=m % 2 == 0)
+
+
+@pytest.mark.parametrize("m,n,k", EVERY_F32)
+def test_every_kernel_fp32(m, n, k):
+    check_linear(m, n, k, torch.float32, bias=m % 2 == 0)
+
+
+@pytest.mark.parametrize("m,n,k", EVERY_GATED)
+def test_every_kernel_gated(m, n, k):
+    check_gated(m, n, k, "gelu" if m % 2 else "silu")
+
+
+@pytest.mark.parametrize("m,k", [(1, 77), (5, 1001), (40, 300), (16, 136), (33, 5001), (3, 20001)])
+def test_nothing_behind_the_last_row(m, k):
+    """Outputs through the C ABI, inside buffers of a known pattern: what lies behind them stays."""
+    from quantization_amd import _native, block_fp8 as F
+    L, st = _native.lib(), torch.cuda.current_stream().cuda_stream
+    n = k + 2                                        # another odd width for the products
+    x = rand(m, k, torch.bfloat16, 1).cuda()
+    r = rand(m, k, torch.bfloat16, 2).cuda()
+    g = torch.ones(k, dtype=torch.bfloat16, device="cuda")
+    (xq, xs), (wq, ws) = F.quantize_blocks_fp8(x), F.quantize_weight_fp8(rand(n, k, torch.float32, 3).cuda())
+
+    def guarded(size):
+        return torch.full((size + 64,), 0xA5, dtype=torch.uint8, device="cuda")
+
+    def kept(*pairs):
+        torch.cuda.synchronize()
+        for buffer, size in pairs:
+            assert bool((buffer[size:] == 0xA5).all()), size
+    kb, nb = (k + 127) // 128, (n + 127) // 128
+    q, s, total = guarded(m * k), guarded(4 * kb * m), guarded(2 * m * k)
+    assert L.miq_quantize_blocks_fp8(x.data_ptr(), 2, m, k, q.data_ptr(), s.data_ptr(), st) == 0
+    kept((q, m * k), (s, 4 * kb * m))
+    assert L.miq_rms_norm_fp8(x.data_ptr(), r.data_ptr(), g.data_ptr(), 2, 2, m, k, 1e-6, total.data_ptr(), q.data_ptr(), s.data_ptr(), st) == 0
+    kept((q, m * k), (s, 4 * kb * m), (total, 2 * m * k))
+    wc, wsc = guarded(m * k), guarded(4 * kb * ((m + 127) // 128))
+    assert L.miq_quantize_weight_fp8(x.data_ptr(), 2, m, k, wc.data_ptr(), wsc.data_ptr(), st) == 0
+    kept((wc, m * k), (wsc, 4 * kb * ((m + 127) // 128)))
+    for code, size in ((0, 4), (1, 2), (2, 2)):
+        need = L.miq_gemm_fp8_workspace(m, n, k, code)
+        work, out = guarded(need), guarded(m * n * size)
+        assert L.miq_gemm_fp8(xq.data_ptr(), xs.data_ptr(), wq.data_ptr(), ws.data_ptr(), m, n, k, None, out.data_ptr(), code,
+                              work.data_ptr(), need, st) == 0
+        kept((work, need), (out, m * n * size))
+    need = L.miq_gated_fp8_workspace(m, n, k)
+    work, out, osc = guarded(need), guarded(m * n), guarded(4 * nb * m)
+    assert L.miq_gated_fp8(xq.data_ptr(), xs.data_ptr(), wq.data_ptr(), ws.data_ptr(), wq.data_ptr(), ws.data_ptr(), m, n, k, 0,
+                           out.data_ptr(), osc.data_ptr(), work.data_ptr(), need, st) == 0
+    kept((work, need), (out, m * n), (osc, 4 * nb * m))
 
 
 # ---- layers ----------------------------------------------------------------------------------------------------------------
