@@ -898,6 +898,8 @@ int check_sizes(const char* who, int64_t M, int64_t N, int64_t K) {
                 "%s: M and N must be below 2^31, K below 2^22 (M=%lld N=%lld K=%lld)", who, (long long)M, (long long)N, (long long)K);
     const int64_t tiles = ceil_div(M, 64) * ceil_div(N, 64);
     MIQ_REQUIRE(tiles <= (1ll << 22), MIQ_ERANGE, "%s: more than 2^22 tiles of 64 x 64 outputs", who);
+    // (at most 16 rows: 512 threads for 16 columns, and a launch holds less than 2^32 threads)
+    MIQ_REQUIRE(M > 16 || N <= (1ll << 26), MIQ_ERANGE, "%s: more than 2^26 columns of at most 16 rows", who);
     return MIQ_OK;
 }
 

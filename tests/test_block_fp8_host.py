@@ -66,6 +66,7 @@ def test_product_refusals():
     for f in (gemm, gated):
         assert f(M=-1) == -1 and f(N=-1) == -1 and f(K=-1) == -1
         assert f(M=BIG) == -5 and f(N=BIG) == -5 and f(K=1 << 22) == -5 and f(M=1 << 20, N=1 << 20) == -5
+        assert f(M=16, N=(1 << 26) + 1) == -5 and f(M=1, N=1 << 28) == -5 and f(M=17, N=(1 << 28) + 1) == -5
         assert f(x=NULL) == -1 and f(xs=NULL) == -1
         assert f(xs=P(4098)) == -2
         assert f(M=0) == 0 and f(N=0) == 0

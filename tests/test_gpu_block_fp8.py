@@ -314,6 +314,87 @@ def test_empty_sizes():
     assert torch.equal(y, torch.arange(5.0, device=dev).expand(3, 5))
 
 
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_no_columns(m):
+    """K == 0: sums of nothing."""
+    from quantization_amd import block_fp8 as F
+    dev = "cuda"
+    x, xs = F.quantize_blocks_fp8(torch.zeros(m, 0, device=dev))
+    w, ws = F.quantize_weight_fp8(torch.zeros(261, 0, device=dev))
+    bias = torch.arange(261.0, device=dev)
+    for out in FLOATS:
+        assert torch.equal(F.linear_fp8(x, xs, w, ws, bias, out), bias.to(out).expand(m, 261))
+    q, s = F.gated_linear_fp8(x, xs, w, ws, w, ws)
+    assert not bool(q.float().any()) and bool((s == 2.0 ** -126).all())
+
+
+def any_codes(rows, cols, seed):
+    """Random codes below 2, of both signs."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    c = torch.randint(0, 256, (rows, cols), dtype=torch.uint8, generator=g, device="cuda")
+    return (c & 0xBF).view(torch.float8_e4m3fn)
+
+
+@pytest.mark.parametrize("m", [4, 40, 300])
+def test_weights_past_32_bits(m):
+    """A weight of 2.3 GB: its last rows' products are those of a copy of these rows."""
+    from quantization_amd import block_fp8 as F
+    n, k = 70000, 32768
+    kb, nb = k // 128, (n + 127) // 128
+    x, w = any_codes(m, k, 1), any_codes(n, k, 2)
+    xs, ws = torch.rand(kb, m, device="cuda") + 0.5, torch.rand(nb, kb, device="cuda") + 0.5
+    first = (n // 128 - 2) * 128
+    tail, tails = w[first:].clone(), ws[first // 128:].clone()
+    xv = x.double() * xs.double().t().repeat_interleave(128, dim=1)
+    wv = tail.double() * tails.double().repeat_interleave(128, dim=0)[:n - first].repeat_interleave(128, dim=1)
+    ref, mag = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    for out in (torch.float32, torch.bfloat16):
+        y = F.linear_fp8(x, xs, w, ws, None, out)[:, first:].double()
+        err = R.product_error(mag, k) + dropped(out, m) * mag
+        assert bool(((y - ref).abs() <= err + torch.finfo(out).eps / 2 * (ref.abs() + err)).all())
+    q, s = F.gated_linear_fp8(x, xs * 1e-3, w, ws, w, ws)
+    v = ref * 1e-3
+    # silu(v) * v: its slope is at most 2.1 |v|, the activation is within 8 units of |v|, three roundings follow
+    a, dv = v * torch.sigmoid(v) * v, R.product_error(mag * 1e-3, k) + 2.0 ** -22 * v.abs()
+    da = 2.1 * dv * (v.abs() + dv) + 8 * 2.0 ** -23 * v * v + 3 * 2.0 ** -24 * a.abs()
+    R.check_codes_of(q[:, first:], s[first // 128:], a.cpu(), da.cpu())
+
+
+def test_activations_past_32_bits():
+    """2.3 thousand million elements: the last rows are those of a copy."""
+    from quantization_amd import block_fp8 as F
+    m, k = 70001, 32768
+    x = torch.empty(m, k, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    last = x[-40:].clone()
+    q, s = F.quantize_blocks_fp8(x)
+    q1, s1 = F.quantize_blocks_fp8(last)
+    assert torch.equal(q[-40:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[:, -40:], s1)
+    w, ws = F.quantize_weight_fp8(torch.randn(96, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)))
+    y, y1 = (F.linear_fp8(a, b, w, ws, None, torch.float32) for a, b in ((q, s), (q1, s1)))
+    kb = torch.arange(k, device="cuda") // 128
+    mag = (q1.double() * s1.double().t()[:, kb]).abs() @ (w.double() * ws.double()[0][kb]).abs().t()
+    assert bool(((y[-40:] - y1).abs() <= 2 * R.product_error(mag, k) + 2.0 ** -23 * y1.abs()).all())
+    del q
+    g = torch.ones(k, dtype=torch.bfloat16, device="cuda")
+    q, s, h = F.rms_norm_fp8(x, g, 1e-6, residual=x)
+    q1, s1, h1 = F.rms_norm_fp8(last, g, 1e-6, residual=last)
+    assert torch.equal(q[-40:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[:, -40:], s1) and torch.equal(h[-40:], h1)
+
+
+def test_outputs_past_32_bits():
+    """2.2 thousand million outputs of one block each: the last rows are those of a copy, bit for bit."""
+    from quantization_amd import block_fp8 as F
+    m, n, k = 66001, 33000, 128
+    x, w = any_codes(m, k, 5), any_codes(n, k, 6)
+    xs, ws = torch.rand(1, m, device="cuda") + 0.5, torch.rand((n + 127) // 128, 1, device="cuda") + 0.5
+    y = F.linear_fp8(x, xs, w, ws)
+    y1 = F.linear_fp8(x[-50:].clone(), xs[:, -50:].contiguous(), w, ws)
+    assert torch.equal(y[-50:], y1)
+    q, s = F.gated_linear_fp8(x, xs, w, ws, w, ws)
+    q1, s1 = F.gated_linear_fp8(x[-50:].clone(), xs[:, -50:].contiguous(), w, ws, w, ws)
+    assert torch.equal(q[-50:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[:, -50:], s1)
+
+
 # ---- together ------------------------------------------------------------------------------------------------------------
 
 def block_weights(k, n, seed, dtype=torch.bfloat16):
