@@ -359,7 +359,16 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gemm_fp8_tile_kerne
 // finishes act(g) * u in fp32, and the quantizer follows.  Bound by the weight's stream: 1x4096x14336 11.3 us (5.2 TB/s),
 // 1x28672x8192 44 us (5.3), the two weights of 1x14336x4096 26 us (4.5); K that is no multiple of 128, so that a row's K-tile
 // is two half lines, 3.3 (9x17784x10032 54 us).
-template <int GROUPS, int kWaves, int DEPTH, int OUT, int ACT>
+//
+// ANY: rows of any length from 16 bytes on, read where they lie: five whole dwords around a chunk, shifted together (sixteen
+// bytes at any address are one load, too, but a slow one: 1x4096x14335 30 us).  A row's last chunk is the sixteen bytes that end
+// it, shifted down, and what would lie behind them are zeros.  (1x4096x14335 16.6 us; through padded copies 33.5.  Rows of whole vectors, 14336: 11.8.)
+// v without its first `drop` bytes, zeros behind them.
+__device__ __forceinline__ v4i drop_front(v4i v, int drop) {
+    typedef unsigned __int128 u128;
+    return drop < 16 ? __builtin_bit_cast(v4i, __builtin_bit_cast(u128, v) >> (8 * drop)) : v4i{0, 0, 0, 0};
+}
+template <int GROUPS, int kWaves, int DEPTH, int OUT, int ACT, bool ANY>
 __global__ __launch_bounds__(64 * kWaves) void gemm_fp8_rows16_kernel(Fp8Args g) {
     constexpr bool GATED = ACT != kNoAct;
     static_assert(!GATED || GROUPS % 2 == 0, "as many of the gate's groups as of the up projection's");
@@ -383,6 +392,27 @@ __global__ __launch_bounds__(64 * kWaves) void gemm_fp8_rows16_kernel(Fp8Args g)
         rw[j] = make_rsrc(g.w[j / kEach] + static_cast<int64_t>(n0 + first) * g.K,
                           left > 0 ? static_cast<uint32_t>(left) * static_cast<uint32_t>(g.K) : 0);
     }
+    // ANY: the lane's rows themselves (past the matrices the last one; what they give is not stored)
+    struct Row {
+        const uint8_t* base;   // from a whole dword on
+        uint32_t shift;        // bytes from there to the row
+    };
+    Row rows[ANY ? GROUPS + 1 : 1] = {};   // of the weights, and of x
+    if constexpr (ANY) {
+        const int mine = lane & 15;
+        auto row_at = [](const uint8_t* p) {
+            const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 3;
+            return Row{p - shift, shift};
+        };
+#pragma unroll
+        for (int j = 0; j < GROUPS; ++j) {
+            const int n = n0 + j % kEach * 16 + mine;
+            rows[j] = row_at(g.w[j / kEach] + static_cast<int64_t>(n < g.N ? n : g.N - 1) * g.K);
+        }
+        rows[GROUPS] = row_at(g.x + static_cast<int64_t>(mine < g.M ? mine : g.M - 1) * g.K);
+    }
+    // The dwords of K-tile kt and the one behind them lie inside every row (the last row may end the tensor).
+    auto inside = [&](int kt) { return (kt + 1) * kTileK + 4 <= g.K; };
     using scalar_floats = const __attribute__((address_space(4))) float*;
     scalar_floats wscale[GATED ? 2 : 1];
 #pragma unroll
@@ -391,17 +421,35 @@ __global__ __launch_bounds__(64 * kWaves) void gemm_fp8_rows16_kernel(Fp8Args g)
     struct Slot {
         Codes w[GROUPS], x;
         float s;   // the scale of row lane & 15
+        uint32_t more[ANY ? GROUPS + 1 : 1][2];   // the dword behind a chunk's four
     };
     auto fill = [&](Slot& s, int kt) {
         const bool in = kt < kt1;
-        const int kfirst = in ? kt * kTileK : 1 << 30;   // (past the slice: past K)
+        if constexpr (ANY) {
+            const int at = in ? kt : kt0;   // (a K-tile past the slice is dropped as a whole)
+            const bool whole = inside(at);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int k = kfirst + h * 64;
-            const uint32_t off = k + cb < g.K ? row + k : kOob;
+            for (int h = 0; h < 2; ++h) {
+                const int k = at * kTileK + h * 64 + cb, last = k < g.K - kChunk ? k : g.K - kChunk;
 #pragma unroll
-            for (int j = 0; j < GROUPS; ++j) s.w[j].c[h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw[j], off, 0, 0));
-            s.x.c[h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 0, 0));
+                for (int j = 0; j <= GROUPS; ++j) {
+                    const uint8_t* p = rows[j].base;
+                    (j < GROUPS ? s.w[j < GROUPS ? j : 0] : s.x).c[h] =
+                        __builtin_bit_cast(v4i, load16<false>(p + (whole ? k : last + static_cast<int>(rows[j].shift))));
+                    s.more[j][h] = *reinterpret_cast<const uint32_t*>(p + (whole ? k + kChunk : 0));
+                }
+            }
+        } else {
+            const int kfirst = in ? kt * kTileK : 1 << 30;   // (past the slice: past K)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = kfirst + h * 64;
+                const uint32_t off = k + cb < g.K ? row + k : kOob;
+#pragma unroll
+                for (int j = 0; j < GROUPS; ++j)
+                    s.w[j].c[h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw[j], off, 0, 0));
+                s.x.c[h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 0, 0));
+            }
         }
         const __amdgpu_buffer_rsrc_t rs =
             make_rsrc(g.xs + static_cast<int64_t>(in ? kt : 0) * g.M, in ? static_cast<uint32_t>(g.M) * 4 : 0);
@@ -416,6 +464,30 @@ __global__ __launch_bounds__(64 * kWaves) void gemm_fp8_rows16_kernel(Fp8Args g)
 #pragma unroll
         for (int u = 0; u < DEPTH; ++u) {
             const int t = kt + u * kWaves, ts = t < kt1 ? t : kt0;   // (a K-tile past the slice: zeros, times some scale)
+            if constexpr (ANY) {
+                if (t < kt1 && inside(t)) {   // (uniform)
+#pragma unroll
+                    for (int j = 0; j <= GROUPS; ++j)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            v4i& v = (j < GROUPS ? ring[u].w[j < GROUPS ? j : 0] : ring[u].x).c[h];
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) {
+                                const uint32_t next = d < 3 ? static_cast<uint32_t>(v[d < 3 ? d + 1 : 3]) : ring[u].more[j][h];
+                                v[d] = static_cast<int>(__builtin_amdgcn_alignbyte(next, static_cast<uint32_t>(v[d]), rows[j].shift));
+                            }
+                        }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int k = t * kTileK + h * 64 + cb, past = t >= kt1 ? kChunk : k - (g.K - kChunk);
+                        if (past <= 0) continue;
+                        ring[u].x.c[h] = drop_front(ring[u].x.c[h], past);
+#pragma unroll
+                        for (int j = 0; j < GROUPS; ++j) ring[u].w[j].c[h] = drop_front(ring[u].w[j].c[h], past);
+                    }
+                }
+            }
             const Widened x = widen(ring[u].x);
 #pragma unroll
             for (int j = 0; j < GROUPS; ++j) add_scaled(acc[j], block_sum(widen(ring[u].w[j]), x), ring[u].s * wscale[j / kEach][ts]);
@@ -906,10 +978,12 @@ int check_sizes(const char* who, int64_t M, int64_t N, int64_t K) {
 size_t align256(int64_t n) { return static_cast<size_t>(round_up(n, 256)); }
 
 // A row length that is no multiple of 16 bytes cannot be staged in 16-byte pieces: both operands are first copied to rows of
-// a multiple of 16, zero-filled (codes of 0 add nothing), at the front of the workspace.
+// a multiple of 16, zero-filled (codes of 0 add nothing), at the front of the workspace.  (The kernel for at most 16 rows stages
+// nothing; it reads rows of at least 16 bytes as they are.)
 int64_t pitch_of(int64_t K) { return round_up(K, kChunk); }
+bool is_padded(int64_t M, int64_t K) { return K % kChunk != 0 && (M > 16 || K < kChunk); }
 size_t padded_bytes(int64_t M, int64_t N, int64_t weights, int64_t K) {
-    return K % kChunk == 0 ? 0 : align256(M * pitch_of(K)) + static_cast<size_t>(weights) * align256(N * pitch_of(K));
+    return is_padded(M, K) ? align256(M * pitch_of(K)) + static_cast<size_t>(weights) * align256(N * pitch_of(K)) : 0;
 }
 // What a product is cut into: which kernel, how K is split, and how much workspace that needs behind the padded operands.
 struct Fp8Plan {
@@ -1060,7 +1134,8 @@ int launch_rows16(const Fp8Plan& p, const Fp8Args& g, hipStream_t st) {
     // Two K-tiles in flight a wave: with four a wave holds 100 registers instead of 58 and fewer fit a SIMD (1 x 4096 x 14336:
     // 11.7 us against 12.6; 1 x 28672 x 8192 44.3 against 47.6).
     const dim3 grid(static_cast<unsigned>(ceil_div(g.N, ACT != kNoAct ? GROUPS * 8 : GROUPS * 16)), p.splits);
-    gemm_fp8_rows16_kernel<GROUPS, 8, 2, OUT, ACT><<<grid, 512, 0, st>>>(g);
+    if (g.K % kChunk) gemm_fp8_rows16_kernel<GROUPS, 8, 2, OUT, ACT, true><<<grid, 512, 0, st>>>(g);
+    else gemm_fp8_rows16_kernel<GROUPS, 8, 2, OUT, ACT, false><<<grid, 512, 0, st>>>(g);
     return check_launch("gemm_fp8_rows16_kernel");
 }
 template <int OUT>
@@ -1112,10 +1187,10 @@ Fp8Args make_args(const uint8_t* x, const float* xs, const uint8_t* w, const flo
     g.ws[1] = ws2;
     g.M = M;
     g.N = static_cast<int>(N);
-    g.K = static_cast<int>(pitch_of(K));
+    g.K = static_cast<int>(is_padded(M, K) ? pitch_of(K) : K);
     g.kblocks = static_cast<int>(ceil_div(K, kTileK));
     g.pitch = static_cast<int>(round_up(N, 8));
-    if (K % kChunk != 0) {
+    if (is_padded(M, K)) {
         PadArgs a{{x, w, w2}, {}, {M, N, w2 ? N : 0}, static_cast<int>(K), g.K};
         for (int o = 0; o < 3; ++o) {
             a.dst[o] = reinterpret_cast<uint8_t*>(at);
@@ -1179,7 +1254,7 @@ extern "C" int miq_gemm_fp8(const uint8_t* x, const float* x_scale, const uint8_
     MIQ_REQUIRE(out && (K == 0 || (x && x_scale && w && w_scale)), MIQ_EINVAL, "miq_gemm_fp8: null pointer");
     MIQ_REQUIRE(aligned(x_scale, 4) && aligned(w_scale, 4) && aligned(bias, 4) && aligned(out, 16), MIQ_EALIGN,
                 "miq_gemm_fp8: scales and bias must be 4-byte, out 16-byte aligned");
-    MIQ_REQUIRE(K % kChunk != 0 || (aligned(x, 16) && aligned(w, 16)), MIQ_EALIGN, "miq_gemm_fp8: x and w must be 16-byte aligned");
+    MIQ_REQUIRE(aligned(x, 16) && aligned(w, 16), MIQ_EALIGN, "miq_gemm_fp8: x and w must be 16-byte aligned");
     const Fp8Plan plan = make_plan(M, N, K, false, out_dtype != MIQ_F32);
     if (int rc = check_workspace("miq_gemm_fp8", padded_bytes(M, N, 1, K) + plan.slabs, workspace, workspace_bytes)) return rc;
     const hipStream_t st = as_stream(stream);
@@ -1206,7 +1281,7 @@ extern "C" int miq_gated_fp8(const uint8_t* x, const float* x_scale, const uint8
                 "miq_gated_fp8: null pointer");
     MIQ_REQUIRE(aligned(x_scale, 4) && aligned(gate_scale, 4) && aligned(up_scale, 4) && aligned(scale, 4) && aligned(q, 16), MIQ_EALIGN,
                 "miq_gated_fp8: scales must be 4-byte, q 16-byte aligned");
-    MIQ_REQUIRE(K % kChunk != 0 || (aligned(x, 16) && aligned(w_gate, 16) && aligned(w_up, 16)), MIQ_EALIGN,
+    MIQ_REQUIRE(aligned(x, 16) && aligned(w_gate, 16) && aligned(w_up, 16), MIQ_EALIGN,
                 "miq_gated_fp8: x and the weights must be 16-byte aligned");
     const Fp8Plan plan = make_plan(M, N, K, true, false);
     if (int rc = check_workspace("miq_gated_fp8", padded_bytes(M, N, 2, K) + plan.slabs, workspace, workspace_bytes)) return rc;

@@ -586,6 +586,18 @@ def test_every_kernel_gated(m, n, k):
     check_gated(m, n, k, "gelu" if m % 2 else "silu")
 
 
+# at most 16 rows of a length that is no multiple of 16, K whole and in slices
+ANY_ROWS = [(1, 300, 17), (16, 45, 31), (5, 70, 4097), (3, 200, 28671), (16, 9000, 129), (1, 10300, 2063), (9, 128, 143), (2, 33, 16385),
+            (16, 515, 1025), (1, 1, 19), (4, 8200, 250)]
+
+
+@pytest.mark.parametrize("m,n,k", ANY_ROWS)
+def test_few_rows_of_any_length(m, n, k):
+    check_linear(m, n, k, torch.float32, bias=True)
+    check_linear(m, n, k, torch.bfloat16)
+    check_gated(m, n, k, "silu")
+
+
 @pytest.mark.parametrize("m,k", [(1, 77), (5, 1001), (40, 300), (16, 136), (33, 5001), (3, 20001)])
 def test_nothing_behind_the_last_row(m, k):
     """Outputs through the C ABI, inside buffers of a known pattern: what lies behind them stays."""
