@@ -351,6 +351,12 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gemm_fp8_tile_kerne
     }
 }
 
+// v without its first `drop` bytes, zeros behind them.
+__device__ __forceinline__ v4i drop_front(v4i v, int drop) {
+    typedef unsigned __int128 u128;
+    return drop < 16 ? __builtin_bit_cast(v4i, __builtin_bit_cast(u128, v) >> (8 * drop)) : v4i{0, 0, 0, 0};
+}
+
 // ---- at most 16 rows: the weight streams once, HBM -> registers ------------------------------------------------------
 // A row group of 16 weight rows is one operand fragment, and nothing is shared between waves, so nothing is staged: a lane
 // loads the chunks that the instructions want from it.  A workgroup of kWaves waves owns GROUPS row groups; wave v sums
@@ -362,12 +368,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gemm_fp8_tile_kerne
 //
 // ANY: rows of any length from 16 bytes on, read where they lie: five whole dwords around a chunk, shifted together (sixteen
 // bytes at any address are one load, too, but a slow one: 1x4096x14335 30 us).  A row's last chunk is the sixteen bytes that end
-// it, shifted down, and what would lie behind them are zeros.  (1x4096x14335 16.6 us; through padded copies 33.5.  Rows of whole vectors, 14336: 11.8.)
-// v without its first `drop` bytes, zeros behind them.
-__device__ __forceinline__ v4i drop_front(v4i v, int drop) {
-    typedef unsigned __int128 u128;
-    return drop < 16 ? __builtin_bit_cast(v4i, __builtin_bit_cast(u128, v) >> (8 * drop)) : v4i{0, 0, 0, 0};
-}
+// it, shifted down, and what would lie behind them are zeros.  (1x4096x14335 16.6 us, through padded copies 33.5; rows of whole
+// vectors, 1x4096x14336, 11.8.)
 template <int GROUPS, int kWaves, int DEPTH, int OUT, int ACT, bool ANY>
 __global__ __launch_bounds__(64 * kWaves) void gemm_fp8_rows16_kernel(Fp8Args g) {
     constexpr bool GATED = ACT != kNoAct;
@@ -998,11 +1000,12 @@ constexpr int64_t kCus = 256;
 
 // Above 16 rows the large kernel and the tile kernel, the latter with tiles of three heights and K in any number of slices, can
 // all run a product: the one with the smallest estimate does.  The estimates' constants are us, fitted to the times of every
-// variant on 227 shapes, M 17 to 7701, N 65 to 28672, K 128 to 28672, 0.6 TFLOP at most (the estimates are within 12% of the times, the choice within 3% of
-// the best variant's time on average).  E.g. 512x2048x2048 bf16: 64-row tiles 9.0, in two slices 14.8, 128-row tiles 17.3, the
-// large kernel 16.3 (64 rows); 254x354x2560 bf16: 32-row tiles in four slices 7.7, 64-row tiles whole 9.0, the large kernel 19.4;
-// gated 2785x669x10032: 128-row tiles in four slices 112, in two 122, the large kernel 143 (128 rows); gated 2773x5456x224: the
-// large kernel 34 (256 rows), 128-row tiles 57; fp32 1000x10001x4000: the large kernel 84 (192 rows), 101 (256), 128-row tiles 97.
+// variant on 227 shapes, M 17 to 7701, N 65 to 28672, K 128 to 28672, 0.6 TFLOP at most: the estimates are within 12% of the
+// times, the choice within 3% of the best variant's on average.  E.g. 512x2048x2048 bf16: 64-row tiles 9.0, in two slices 14.8,
+// 128-row tiles 17.3, the large kernel 16.3 (64 rows); 254x354x2560 bf16: 32-row tiles in four slices 7.7, 64-row tiles whole 9.0,
+// the large kernel 19.4; gated 2785x669x10032: 128-row tiles in four slices 112, in two 122, the large kernel 143 (128 rows);
+// gated 2773x5456x224: the large kernel 34 (256 rows), 128-row tiles 57; fp32 1000x10001x4000: the large kernel 84 (192 rows), 101
+// (256), 128-row tiles 97.
 struct BigFit {
     double k_tile, round;
 };
