@@ -143,29 +143,44 @@ __device__ __forceinline__ void store4(void* out, int64_t i, int n, bool vec, v4
 // Memory requests before this stay before it, those after it after: the counted waits below depend on the order of issue.
 __device__ __forceinline__ void keep_order() { asm volatile("" ::: "memory"); }
 
-// Rows of K bytes -> rows of `pitch` bytes (K rounded up to 16), zeros past K: one thread a 16-byte piece, up to three
-// matrices in one launch.
+// v without its first `drop` bytes, zeros behind them.
+__device__ __forceinline__ v4i drop_front(v4i v, int drop) {
+    typedef unsigned __int128 u128;
+    return drop < 16 ? __builtin_bit_cast(v4i, __builtin_bit_cast(u128, v) >> (8 * drop)) : v4i{0, 0, 0, 0};
+}
+
+// Rows of K bytes -> rows of `pitch` bytes (K rounded up to 16), zeros past K, up to three matrices in one launch.  A wave takes a
+// row, a lane a 16-byte piece: five whole dwords shifted together, where these lie inside the row; the pieces at its end are the
+// row's last sixteen bytes, shifted down.  (2000 + 2000 rows of 1001 bytes 5.6 us, one thread a piece of any row, loaded at any
+// address, 8.2; 14336 rows of 4095 19.7 and 26.4 us, 5.9 TB/s read and written.)
 struct PadArgs {
-    const uint8_t* src[3];
+    const uint8_t* src[3];   // 4-byte aligned
     uint8_t* dst[3];
     int64_t rows[3];   // 0: none
     int K, pitch;
 };
 __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs a) {
-    const int per_row = a.pitch / kChunk;
-#pragma unroll
-    for (int o = 0; o < 3; ++o) {
-        for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < a.rows[o] * per_row; i += gridDim.x * 256ll) {
-            const int64_t r = i / per_row;
-            const int k = static_cast<int>(i % per_row) * kChunk;
-            const uint8_t* p = a.src[o] + r * a.K + k;
+    const int lane = threadIdx.x & 63, o = blockIdx.y;
+    for (int64_t r = blockIdx.x * 4ll + (threadIdx.x >> 6); r < a.rows[o]; r += gridDim.x * 4ll) {
+        const uint8_t* const row = a.src[o] + r * a.K;
+        const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row)) & 3;
+        v4i* const to = reinterpret_cast<v4i*>(a.dst[o] + r * a.pitch);
+#pragma unroll 4
+        for (int k = lane * kChunk; k < a.K; k += 64 * kChunk) {
             v4i v = {0, 0, 0, 0};
-            if (a.K - k >= kChunk) {
-                __builtin_memcpy(&v, p, kChunk);
+            if (k + kChunk + 4 <= a.K) {
+                const uint8_t* const p = row - shift + k;
+                const u32x4 d = load16<false>(p);
+                const uint32_t e = *reinterpret_cast<const uint32_t*>(p + kChunk);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = static_cast<int>(__builtin_amdgcn_alignbyte(i < 3 ? d[i < 3 ? i + 1 : 3] : e, d[i], shift));
+            } else if (a.K >= kChunk) {
+                const int last = k < a.K - kChunk ? k : a.K - kChunk;
+                v = drop_front(__builtin_bit_cast(v4i, load16<false>(row + last)), k - last);
             } else {
-                for (int b = 0; b < a.K - k; ++b) v[b >> 2] |= static_cast<int>(static_cast<uint32_t>(p[b]) << (8 * (b & 3)));
+                for (int b = 0; b < a.K; ++b) v[b >> 2] |= static_cast<int>(static_cast<uint32_t>(row[b]) << (8 * (b & 3)));
             }
-            *reinterpret_cast<v4i*>(a.dst[o] + i * kChunk) = v;
+            to[k / kChunk] = v;
         }
     }
 }
@@ -349,12 +364,6 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gemm_fp8_tile_kerne
                 if (n < cols && m + r < g.M) store_value<OUT>(out, (m + r) * cols + n, v[r / kStep]);
         }
     }
-}
-
-// v without its first `drop` bytes, zeros behind them.
-__device__ __forceinline__ v4i drop_front(v4i v, int drop) {
-    typedef unsigned __int128 u128;
-    return drop < 16 ? __builtin_bit_cast(v4i, __builtin_bit_cast(u128, v) >> (8 * drop)) : v4i{0, 0, 0, 0};
 }
 
 // ---- at most 16 rows: the weight streams once, HBM -> registers ------------------------------------------------------
@@ -1202,8 +1211,8 @@ Fp8Args make_args(const uint8_t* x, const float* xs, const uint8_t* w, const flo
         g.x = a.dst[0];
         g.w[0] = a.dst[1];
         if (w2) g.w[1] = a.dst[2];
-        const int64_t groups = ceil_div((M > N ? M : N) * (g.K / kChunk), 256);
-        pad_rows_kernel<<<static_cast<unsigned>(groups < 16384 ? groups : 16384), 256, 0, st>>>(a);
+        const int64_t groups = ceil_div(M > N ? M : N, 4);
+        pad_rows_kernel<<<dim3(static_cast<unsigned>(groups < 16384 ? groups : 16384), w2 ? 3 : 2), 256, 0, st>>>(a);
     }
     return g;
 }
