@@ -173,7 +173,8 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs a) {
                 const u32x4 d = load16<false>(p);
                 const uint32_t e = *reinterpret_cast<const uint32_t*>(p + kChunk);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = static_cast<int>(__builtin_amdgcn_alignbyte(i < 3 ? d[i < 3 ? i + 1 : 3] : e, d[i], shift));
+                for (int i = 0; i < 4; ++i)
+                    v[i] = static_cast<int>(__builtin_amdgcn_alignbyte(i < 3 ? d[i < 3 ? i + 1 : 3] : e, d[i], shift));
             } else if (a.K >= kChunk) {
                 const int last = k < a.K - kChunk ? k : a.K - kChunk;
                 v = drop_front(__builtin_bit_cast(v4i, load16<false>(row + last)), k - last);
@@ -371,7 +372,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gemm_fp8_tile_kerne
 // loads the chunks that the instructions want from it.  A workgroup of kWaves waves owns GROUPS row groups; wave v sums
 // the K-tiles v, v + kWaves, ... (eight consecutive K-tiles are 1 KiB of a row), DEPTH of them in flight, and the partial
 // sums meet in LDS.  A gated product's groups are the gate's and the up projection's of the same columns: the workgroup
-// finishes act(g) * u in fp32, and the quantizer follows.  Bound by the weight's stream: 1x4096x14336 11.3 us (5.2 TB/s),
+// finishes act(g) * u in fp32, and the quantizer follows (a workgroup that has a whole block's 128 columns could quantize it
+// itself, but streams them alone: 1x4096x1024 12.6 us for 6.1, 1x14336x4096 44 for 30).  Bound by the weight's stream: 1x4096x14336 11.3 us (5.2 TB/s),
 // 1x28672x8192 44 us (5.3), the two weights of 1x14336x4096 26 us (4.5); K that is no multiple of 128, so that a row's K-tile
 // is two half lines, 3.3 (9x17784x10032 54 us).
 //
