@@ -836,8 +836,9 @@ def _float_matrix(x, name):
 
 def _codes_matrix(q, scale, index, name, weight):
     """(rows, columns) of a dense matrix of codes whose scales are those of an activation or of a weight."""
-    _require(q, index, name)
-    _require(scale, index, f"the scales of {name}")
+    if not (q.get_device() == scale.get_device() == index and q.is_contiguous() and scale.is_contiguous()):
+        _require(q, index, name)
+        _require(scale, index, f"the scales of {name}")
     if q.dtype is not _F8 or q.dim() != 2:
         raise RuntimeError(f"{name} must be a float8_e4m3fn matrix, got {tuple(q.shape)} {q.dtype}")
     r, c = q.shape

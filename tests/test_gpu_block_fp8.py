@@ -194,7 +194,7 @@ LARGE = [(2048, 4100, 272), (300, 16260, 130), (1025, 6500, 1040)]
 @pytest.mark.parametrize("out", FLOATS)
 @pytest.mark.parametrize("m,n,k", LARGE)
 def test_large_linear(out, m, n, k):
-    """Sizes of at least 128 tiles of 256 x 256."""
+    """Many tiles, ragged ones at the edges, and a K that ends inside a block."""
     from quantization_amd import block_fp8 as F
     xq, xs = codes(m, k, 1)
     wq, ws = codes(n, k, 2, weight=True)
@@ -228,7 +228,7 @@ def test_large_gated(act, m, n, k):
     R.check_codes_of(q[keep], s[:, keep], y, dy)
 
 
-# at most 64 rows against many blocks of 128 columns: one launch
+# at most 64 rows against many blocks of 128 columns
 FEW = [(1, 10240, 128), (1, 10300, 2064), (3, 10241, 130), (16, 10240, 640), (17, 10368, 1000), (33, 10250, 272), (48, 10240, 520), (64, 10300, 384)]
 
 
