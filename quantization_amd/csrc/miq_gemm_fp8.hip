@@ -1059,9 +1059,9 @@ Fp8Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated, bool native) {
     const int64_t nt = ceil_div(K, kTileK);
     const int64_t slab = 4 * M * round_up(N, 8);
     if (M <= 16) {
-        // A slice of K to every eighth workgroup's worth of K-tiles where the columns give few workgroups and K is long enough to
-        // pay for the second launch: 1x512x28672 18.3 us whole, 8.0 in eight slices, 1x512x14336 11.2 and 6.6 (and 4 us more of
-        // the host), 1x2048x8192 7.4 and 8.3.  A gated product has its second launch anyway and would have a third.
+        // K in slices of at least eight K-tiles where the columns give few workgroups and K is long enough to pay for the second
+        // launch: 1x512x28672 18.3 us whole, 8.0 in eight slices, 1x512x14336 11.2 and 6.6 (and 4 us more of the host), 1x2048x8192
+        // 7.4 and 8.3.  A gated product has its second launch anyway and would have a third (8x2048x4096 10.7 us, sliced 12.9).
         const int64_t groups = ceil_div(N, 16);
         if (!gated && groups < 192 && nt >= 128) {
             int64_t splits = kCus / groups;
@@ -1104,13 +1104,7 @@ Fp8Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated, bool native) {
             p.kt_per_split = static_cast<int>(slices > 1 || gated ? (kt > 0 ? kt : 1) : 0);   // gated: one slab a weight at least
         }
     }
-    if (p.big) {
-        p.bm = 0;
-        p.splits = 1;
-        p.kt_per_split = 0;
-    } else if (gated || p.splits > 1) {
-        p.slabs = static_cast<size_t>(products * p.splits * slab);
-    }
+    if (!p.big && (gated || p.splits > 1)) p.slabs = static_cast<size_t>(products * p.splits * slab);
     return p;
 }
 
