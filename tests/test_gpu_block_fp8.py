@@ -586,6 +586,37 @@ def test_every_kernel_gated(m, n, k):
     check_gated(m, n, k, "gelu" if m % 2 else "silu")
 
 
+# sizes of every kernel that a gated product can run by, a last block of one column among them
+GELU_TAILS = [(1, 1, 16), (5, 129, 64), (16, 257, 2063), (40, 129, 64), (19, 80, 432), (90, 5584, 64), (3754, 130, 64), (4182, 72, 4224), (2330, 65, 1040),
+              (2308, 784, 64), (8294, 417, 64), (446, 11192, 64), (1000, 2000, 1000)]
+
+
+@pytest.mark.parametrize("m,n,k", GELU_TAILS)
+def test_gelu_of_negative_gates(m, n, k):
+    """Gates between -13.2 and -2.2 in whole blocks, where 1 + erf(g / sqrt 2) is what rounding leaves of 1 - 1: the activation
+    keeps its relative accuracy.  A row has one column that is not zero, so that the gate is one exact product of two codes.
+
+    With t = -g / sqrt 2 in fp32 (its constant and its product rounded: 2^-24 relative each), erfc(t) moves by its slope, at most
+    (g^2 + 1) times that; the function itself is within 8 units, three products follow."""
+    from quantization_amd import block_fp8 as F
+    gen = torch.Generator(device="cuda").manual_seed(m + n + k)
+
+    def picks(values, *shape):
+        v = torch.tensor(values, device="cuda")
+        return v[torch.randint(0, len(values), shape, generator=gen, device="cuda")]
+    x = torch.zeros(m, k, device="cuda")
+    col = torch.randint(0, k, (m,), generator=gen, device="cuda")
+    x[torch.arange(m, device="cuda"), col] = picks([1.0, 1.125, 1.25, 1.5, 1.75, 1.875], m)
+    w, u = picks([-2.25, -4.0, -4.5, -5.0, -5.5, -6.0, -6.5, -7.0], n, k), picks([-3.0, -1.125, 0.5, 1.0, 2.5], n, k)
+    xs, ws = torch.ones((k + 127) // 128, m, device="cuda"), torch.ones((n + 127) // 128, (k + 127) // 128, device="cuda")
+    q, s = F.gated_linear_fp8(x.to(torch.float8_e4m3fn), xs, w.to(torch.float8_e4m3fn), ws, u.to(torch.float8_e4m3fn), ws, "gelu")
+    xv = x[torch.arange(m, device="cuda"), col].double()[:, None]
+    g, uv = xv * w[:, col].t().double(), xv * u[:, col].t().double()
+    y = 0.5 * g * torch.special.erfc(g * -math.sqrt(0.5)) * uv   # (torch's ndtr is 1 + erf itself: 0 from -8.3 on in 64 bits)
+    dy = ((g * g + 1) * 2.0 ** -23 + 8 * 2.0 ** -23 + 3 * 2.0 ** -24) * y.abs()
+    R.check_codes_of(q, s, y.cpu(), dy.cpu())
+
+
 # at most 16 rows of a length that is no multiple of 16, K whole and in slices
 ANY_ROWS = [(1, 300, 17), (16, 45, 31), (5, 70, 4097), (3, 200, 28671), (16, 9000, 129), (1, 10300, 2063), (9, 128, 143), (2, 33, 16385),
             (16, 515, 1025), (1, 1, 19), (4, 8200, 250)]
