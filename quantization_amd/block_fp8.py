@@ -94,7 +94,7 @@ class BlockFP8Linear(_BlockFP8Module):
         self.out_dtype = out_dtype
         self.register_buffer("weight", weight)
         self.register_buffer("weight_scale", weight_scale)
-        self.register_buffer("bias", None if bias is None else bias.detach().to(torch.float32).contiguous())
+        self.register_buffer("bias", None if bias is None else bias.detach().to(torch.float32, copy=True).contiguous())
 
     @classmethod
     def from_float(cls, module, out_dtype=None):

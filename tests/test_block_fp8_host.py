@@ -89,6 +89,21 @@ def test_wrappers_refuse_host_tensors():
             call()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_layer_owns_its_bias(dtype):
+    """A layer built from a float one shares no storage with it: loading a state into the one leaves the other as it is."""
+    from quantization_amd import block_fp8 as F
+    lin = torch.nn.Linear(6, 3).to(dtype)
+    before = lin.bias.detach().clone()
+    layer = F.BlockFP8Linear(torch.zeros(3, 6).to(torch.float8_e4m3fn), torch.ones(1, 1), lin.bias)
+    assert layer.bias.dtype == torch.float32 and torch.equal(layer.bias, before.float()) and not layer.bias.requires_grad
+    layer.load_state_dict({"weight": layer.weight, "weight_scale": layer.weight_scale, "bias": torch.full((3,), 7.0)})
+    assert torch.equal(lin.bias.detach(), before)
+    with torch.no_grad():
+        lin.bias.fill_(5.0)
+    assert torch.equal(layer.bias, torch.full((3,), 7.0))
+
+
 @pytest.mark.gpu
 def test_wrappers_refuse_wrong_tensors():
     from quantization_amd import block_fp8 as F
