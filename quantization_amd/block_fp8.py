@@ -86,7 +86,7 @@ class _BlockFP8Module(nn.Module):
 
 class BlockFP8Linear(_BlockFP8Module):
     """nn.Linear on block-scaled e4m3 codes.  forward() takes a float tensor (which it quantizes) or a pair (codes, scales); its
-    output is of the tensor's type, bfloat16 for a pair, or of out_dtype where one is given."""
+    output is of the layer's out_dtype, of forward()'s where the layer has none, else of the tensor's type, bfloat16 for a pair."""
 
     def __init__(self, weight, weight_scale, bias=None, out_dtype=None):
         super().__init__()
@@ -102,9 +102,9 @@ class BlockFP8Linear(_BlockFP8Module):
         home = module.weight.device
         return cls(w.to(home), scale.to(home), module.bias, out_dtype)
 
-    def forward(self, x):
+    def forward(self, x, out_dtype=None):
         q, scale, dtype = self._codes(x)
-        return linear_fp8(q, scale, self.weight, self.weight_scale, self.bias, self.out_dtype or dtype)
+        return linear_fp8(q, scale, self.weight, self.weight_scale, self.bias, self.out_dtype or out_dtype or dtype)
 
     def extra_repr(self):
         return f"{self.in_features}, {self.out_features}, bias={self.bias is not None}"
@@ -113,7 +113,8 @@ class BlockFP8Linear(_BlockFP8Module):
 class BlockFP8GatedMLP(_BlockFP8Module):
     """down(act(gate(x)) * up(x)) on block-scaled e4m3 codes, 8 bits between the products: two launches for a prompt (the
     gated product ends in codes), one more to quantize a float input.  forward() takes what BlockFP8Linear takes; rms_norm_fp8
-    makes such a pair of a layer's input."""
+    makes such a pair of a layer's input.  `down` is called as a module, down((codes, scales), out_dtype=the type to answer in),
+    so that its hooks run and another module may stand in its place."""
 
     def __init__(self, gate, gate_scale, up, up_scale, down, act="silu"):
         super().__init__()
@@ -137,4 +138,4 @@ class BlockFP8GatedMLP(_BlockFP8Module):
     def forward(self, x):
         q, scale, dtype = self._codes(x)
         hidden = gated_linear_fp8(q, scale, self.gate, self.gate_scale, self.up, self.up_scale, self.act)
-        return linear_fp8(*hidden, self.down.weight, self.down.weight_scale, self.down.bias, self.down.out_dtype or dtype)
+        return self.down(hidden, out_dtype=dtype)

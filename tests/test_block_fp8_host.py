@@ -104,6 +104,30 @@ def test_layer_owns_its_bias(dtype):
     assert torch.equal(layer.bias, torch.full((3,), 7.0))
 
 
+def test_gated_layer_calls_its_down_projection(monkeypatch):
+    """Hooks on `down` run, and a module put in its place is what is called, with the pair and the type to answer in."""
+    from quantization_amd import block_fp8 as F
+    f8, pair = torch.zeros(4, 6).to(torch.float8_e4m3fn), (torch.zeros(2, 4).to(torch.float8_e4m3fn), torch.ones(1, 2))
+    monkeypatch.setattr(F, "quantize_blocks_fp8", lambda x: (x.to(torch.float8_e4m3fn), torch.ones(1, 2)))
+    monkeypatch.setattr(F, "gated_linear_fp8", lambda *a: pair)
+    monkeypatch.setattr(F, "linear_fp8", lambda q, s, w, ws, b, dtype: torch.zeros(2, w.shape[0], dtype=dtype))
+    down = F.BlockFP8Linear(torch.zeros(6, 4).to(torch.float8_e4m3fn), torch.ones(1, 1))
+    mlp = F.BlockFP8GatedMLP(f8, torch.ones(1, 1), f8, torch.ones(1, 1), down)
+    seen = []
+    down.register_forward_hook(lambda module, args, out: seen.append(args) or out + 1)
+    y = mlp(torch.zeros(2, 6, dtype=torch.float16))
+    assert len(seen) == 1 and seen[0][0] is pair and y.dtype == torch.float16 and bool((y == 1).all())
+    assert mlp(pair).dtype == torch.bfloat16 and mlp(torch.zeros(2, 6)).dtype == torch.float32
+    down.out_dtype = torch.float32
+    assert mlp(pair).dtype == torch.float32 and mlp(torch.zeros(2, 6).half()).dtype == torch.float32
+
+    class Other(torch.nn.Module):
+        def forward(self, x, out_dtype):
+            return x, out_dtype
+    mlp.down = Other()
+    assert mlp(torch.zeros(2, 6).half()) == (pair, torch.float16)
+
+
 @pytest.mark.gpu
 def test_wrappers_refuse_wrong_tensors():
     from quantization_amd import block_fp8 as F
