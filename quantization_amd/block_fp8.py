@@ -73,7 +73,10 @@ class _BlockFP8Module(nn.Module):
         def moved(t):
             new = fn(t)
             return new if new.dtype == t.dtype else t.to(new.device)
-        return super()._apply(moved, recurse)
+        if recurse:
+            for child in self.children():   # by their own rule
+                child._apply(fn)
+        return super()._apply(moved, recurse=False)
 
     @staticmethod
     def _codes(x):

@@ -128,6 +128,21 @@ def test_gated_layer_calls_its_down_projection(monkeypatch):
     assert mlp(torch.zeros(2, 6).half()) == (pair, torch.float16)
 
 
+def test_gated_layer_casts_another_down_projection():
+    """Codes and scales keep their types in a cast of the model; a float module in the place of `down` is cast as any other."""
+    from quantization_amd import block_fp8 as F
+    f8 = torch.zeros(4, 6).to(torch.float8_e4m3fn)
+    mlp = F.BlockFP8GatedMLP(f8, torch.ones(1, 1), f8, torch.ones(1, 1), F.BlockFP8Linear(f8, torch.ones(1, 1), torch.zeros(4)))
+    mlp.half()
+    assert {n: b.dtype for n, b in mlp.named_buffers()} == {
+        "gate": f8.dtype, "gate_scale": torch.float32, "up": f8.dtype, "up_scale": torch.float32, "down.weight": f8.dtype,
+        "down.weight_scale": torch.float32, "down.bias": torch.float32}
+    mlp.down = torch.nn.Linear(4, 6)
+    mlp.to(torch.bfloat16)
+    assert mlp.gate.dtype == f8.dtype and mlp.gate_scale.dtype == torch.float32
+    assert mlp.down.weight.dtype == mlp.down.bias.dtype == torch.bfloat16
+
+
 @pytest.mark.gpu
 def test_wrappers_refuse_wrong_tensors():
     from quantization_amd import block_fp8 as F
