@@ -134,7 +134,7 @@ def test_gated_layer_casts_another_down_projection():
     f8 = torch.zeros(4, 6).to(torch.float8_e4m3fn)
     mlp = F.BlockFP8GatedMLP(f8, torch.ones(1, 1), f8, torch.ones(1, 1), F.BlockFP8Linear(f8, torch.ones(1, 1), torch.zeros(4)))
     mlp.half()
-    assert {n: b.dtype for n, b in mlp.named_buffers()} == {
+    assert {n: b.dtype for n, b in mlp.named_buffers(remove_duplicate=False)} == {   # (one tensor of codes for all three)
         "gate": f8.dtype, "gate_scale": torch.float32, "up": f8.dtype, "up_scale": torch.float32, "down.weight": f8.dtype,
         "down.weight_scale": torch.float32, "down.bias": torch.float32}
     mlp.down = torch.nn.Linear(4, 6)
