@@ -409,6 +409,8 @@ int miq_quantize_weight_fp8(const void* w, int w_dtype, int64_t N, int64_t K, ui
  *     h = x + residual (rounded to dtype; h = x without a residual)       sum = h (written when there is a residual)
  *     y[m,k] = (h[m,k] * (1 / sqrt(mean_k h[m,k]^2 + eps))) * weight[k]   fp32
  *     q, scale = the codes of y
+ * Finite rows of any size: where the sum of squares leaves fp32's range (or lies too low in it for eps to cover) the row is taken
+ * times a power of two first.  A row of zeros gives codes of 0, with eps = 0 too.
  * x, residual, sum: [M,K] of dtype; residual and sum are both null or both given.  weight: [K] of weight_dtype, which is
  * dtype or MIQ_F32. */
 int miq_rms_norm_fp8(const void* x, const void* residual, const void* weight, int dtype, int weight_dtype, int64_t M, int64_t K,

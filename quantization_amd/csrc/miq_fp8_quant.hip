@@ -162,7 +162,8 @@ template <int DT, bool VEC, int TPR, int VPT>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(NormArgs a) {
     constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR, kWaves = TPR / 64;
     constexpr int kKeep = VPT > 0 ? VPT : 1;
-    __shared__ float part[kThreads / 64];
+    __shared__ float part[kWaves];
+    __shared__ uint32_t tops[kWaves];
     const int t = threadIdx.x % TPR;
     const int64_t m = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
     const bool live = m < a.M;
@@ -180,42 +181,28 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(NormArg
             if (write) store8<DT, VEC>(a.sum, row + k, n, h);
         }
     };
-    float h[kKeep][8];
     float ss = 0.0f;
-    if constexpr (VPT > 0) {
+    auto add_squares = [&](const float (&v)[8]) {
+        float s8 = 0.0f;
 #pragma unroll
-        for (int v = 0; v < VPT; ++v) {
-            const int64_t k = (static_cast<int64_t>(v) * TPR + t) * 8;
-            load_h(k, count(k), h[v], true);
-        }
+        for (int i = 0; i < 8; ++i) s8 = __fadd_rn(s8, __fmul_rn(v[i], v[i]));
+        ss += s8;
+    };
+    auto over_row = [&](auto v, auto* of_wave, auto join) {
 #pragma unroll
-        for (int v = 0; v < VPT; ++v) {
-            float s8 = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s8 = __fadd_rn(s8, __fmul_rn(h[v][i], h[v][i]));
-            ss += s8;
-        }
-    } else {
-        for (int64_t v = 0; v < rounds; ++v) {
-            const int64_t k = (v * TPR + t) * 8;
-            load_h(k, count(k), h[0], true);
-            float s8 = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s8 = __fadd_rn(s8, __fmul_rn(h[0][i], h[0][i]));
-            ss += s8;
-        }
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-    if constexpr (kWaves > 1) {
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ss;
+        for (int o = 32; o > 0; o >>= 1) v = join(v, __shfl_xor(v, o, 64));
+        if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = v;
         __syncthreads();
-        ss = 0.0f;
+        v = of_wave[0];
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) ss += part[i];
-    }
-    const float inv_rms = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(a.K)), a.eps)));
-    auto finish = [&](int64_t k, int n, float (&hv)[8]) {
+        for (int i = 1; i < kWaves; ++i) v = join(v, of_wave[i]);
+        return v;
+    };
+    auto plus = [](float a, float b) { return a + b; };
+    auto inverse_rms = [&](float eps) {
+        return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(a.K)), eps)));
+    };
+    auto finish = [&](int64_t k, int n, float (&hv)[8], float inv_rms) {
         float g[8];
         if (DT == MIQ_F32 || a.g_f32) load8<MIQ_F32, VEC, false>(a.g, k, k < a.K ? (a.K - k < 8 ? a.K - k : 8) : 0, g);
         else load8<DT, VEC, false>(a.g, k, k < a.K ? (a.K - k < 8 ? a.K - k : 8) : 0, g);
@@ -226,18 +213,67 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(NormArg
         store8_codes<VEC>(a.q, row + k, n, c);
         if ((threadIdx.x & 15) == 0 && n > 0) a.scale[(k / kBlockK) * a.M + m] = s;
     };
+    // The vectors of the row times 2^-shift, read one by one.
+    auto each_vector = [&](int shift, bool write, auto use) {
+        for (int64_t v = 0; v < rounds; ++v) {
+            const int64_t k = (v * TPR + t) * 8;
+            float h[8];
+            load_h(k, count(k), h, write);
+            if (shift) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[i] = ldexpf(h[i], -shift);
+            }
+            use(k, h);
+        }
+    };
+    float h[kKeep][8];
     if constexpr (VPT > 0) {
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
             const int64_t k = (static_cast<int64_t>(v) * TPR + t) * 8;
-            finish(k, count(k), h[v]);
+            load_h(k, count(k), h[v], true);
+        }
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) add_squares(h[v]);
+    } else {
+        each_vector(0, true, [&](int64_t, float (&hv)[8]) { add_squares(hv); });
+    }
+    ss = over_row(ss, part, plus);
+    // The sum of squares of a finite row can pass fp32's range (bf16 and fp32 rows from some 1e18 on), or lie where squares lose
+    // bits and eps does not cover them.  Such a row (the same finding in every thread) is read again and taken times the power of
+    // two that puts its largest value between 1 and 2, which is exact; 2^120 at most, so that eps times its square is finite.
+    if (!(ss < __builtin_inff()) || (ss < 0x1p-90f && a.eps < 0x1p-120f)) {
+        uint32_t top = 0;
+        each_vector(0, false, [&](int64_t, float (&hv)[8]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t b = magnitude_bits(hv[i]);
+                top = b > top ? b : top;
+            }
+        });
+        top = over_row(top, tops, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+        const int exponent = static_cast<int>(top >> 23) - 127;
+        // (an infinity or a NaN: as they are)
+        const int shift = top == 0 || top >= kInfBits ? 0 : exponent > -120 ? exponent : -120;
+        if (shift) {
+            ss = 0.0f;
+            each_vector(shift, false, [&](int64_t, float (&hv)[8]) { add_squares(hv); });
+            ss = over_row(ss, part, plus);
+        }
+        // (a row of zeros without eps has no norm: its codes are 0)
+        const float inv_rms = top == 0 && a.eps == 0.0f ? 1.0f : inverse_rms(ldexpf(a.eps, -2 * shift));
+        each_vector(shift, false, [&](int64_t k, float (&hv)[8]) { finish(k, count(k), hv, inv_rms); });
+        return;
+    }
+    const float inv_rms = inverse_rms(a.eps);
+    if constexpr (VPT > 0) {
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int64_t k = (static_cast<int64_t>(v) * TPR + t) * 8;
+            finish(k, count(k), h[v], inv_rms);
         }
     } else {
-        for (int64_t v = 0; v < rounds; ++v) {
-            const int64_t k = (v * TPR + t) * 8;
-            load_h(k, count(k), h[0], false);
-            finish(k, count(k), h[0]);
-        }
+        each_vector(0, false, [&](int64_t k, float (&hv)[8]) { finish(k, count(k), hv, inv_rms); });
     }
 }
 

@@ -153,6 +153,50 @@ def test_rms_norm_empty_mask_rows_and_spoiled_rows():
     R.check_codes_of(q[keep], s[:, keep], y, dy)
 
 
+@pytest.mark.parametrize("dtype,size", [(torch.bfloat16, 3e18), (torch.bfloat16, 3e38), (torch.float32, 2e19), (torch.float32, 1e37),
+                                        (torch.float32, 1e-20), (torch.float32, 3e-24), (torch.bfloat16, 1e-36), (torch.float32, 1e-43)])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("m,k", [(3, 1), (3, 300), (3, 2056), (2, 5000), (2, 16384), (2, 16392), (2, 40001)])
+def test_rms_norm_of_far_values(dtype, size, residual, m, k):
+    """Finite rows whose squares are beyond fp32's range, or below it where eps does not cover them; one row is ordinary, another
+    has the largest value alone among small ones.  (A power of two from the row's largest value goes through every step exactly.)"""
+    from quantization_amd import block_fp8 as F
+    eps = 1e-6 if size > 1 else 0.0
+    x = torch.rand(m, k, generator=torch.Generator().manual_seed(k)).mul_(0.75).add_(0.25)
+    x *= torch.where(torch.rand(m, k, generator=torch.Generator().manual_seed(k + 1)) < 0.5, -1.0, 1.0)
+    x[0] *= size
+    x[1, 0] = size
+    x = x.to(dtype)
+    r = (x.float() * 0.125).to(dtype) if residual else None
+    g = (1 + 0.2 * torch.randn(k, generator=torch.Generator().manual_seed(k))).to(dtype)
+    got = F.rms_norm_fp8(x.cuda(), g.cuda(), eps, residual=None if r is None else r.cuda())
+    y, dy, total = norm_reference(x, g, eps, r)
+    R.check_codes_of(got[0], got[1], y, dy + 2.0 ** -140)   # (scaled values below 2^-126: 2^-150, times at most 2^8 for 1 / rms and 2 for g)
+    if residual:
+        assert torch.equal(got[2].cpu(), total)
+
+
+@pytest.mark.parametrize("k", [300, 40001])
+def test_rms_norm_without_eps(k):
+    """A row of zeros has no norm: its codes are 0 whatever eps is.  Infinities and NaN as ever: a NaN in its whole row; an
+    infinity is a NaN code, and what it is the norm of is 0 elsewhere."""
+    from quantization_amd import block_fp8 as F
+    x = rand(5, k, torch.float32, 3)
+    x[0] = 0
+    x[2, 17] = math.nan
+    x[3, 200] = -math.inf
+    x[3, 7] = 3e38
+    g = torch.ones(k)
+    for eps in (0.0, 1e-6):
+        q, s = F.rms_norm_fp8(x.cuda(), g.cuda(), eps)
+        assert not bool(q[0].float().any()) and bool((s[:, 0] == 2.0 ** -126).all())
+        assert bool(torch.isnan(q[2].float()).all())
+        nan = torch.isnan(q[3].float())
+        assert bool(nan[200]) and int(nan.sum()) == 1 and not bool(q[3].float()[~nan].any())
+        y, dy, _ = norm_reference(x[[1, 4]], g, eps, None)
+        R.check_codes_of(q[[1, 4]], s[:, [1, 4]], y, dy)
+
+
 # ---- products ----------------------------------------------------------------------------------------------------------
 
 PRODUCTS = [(1, 1, 1), (1, 64, 16), (1, 130, 4096), (2, 129, 100), (7, 300, 1000), (15, 257, 1024), (16, 128, 128), (17, 640, 2064),
