@@ -47,6 +47,8 @@ def quantize_weight_fp8(w):
 def rms_norm_fp8(x, weight, eps=1e-6, residual=None):
     """The codes of h / rms(h) * weight, with h = x (returns codes, scales) or, with a residual, h = x + residual rounded to
     x's type (returns codes, scales, h).  weight: [K] of x's type or float32."""
+    if residual is not None and residual.shape != x.shape:
+        raise RuntimeError(f"residual must be {tuple(x.shape)}, got {tuple(residual.shape)}")
     q, scale, total = _native.rms_norm_fp8(_rows(x), weight, eps, None if residual is None else _rows(residual))
     if x.dim() != 2:
         q, total = q.view(x.shape), None if total is None else total.view(x.shape)

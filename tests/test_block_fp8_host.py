@@ -143,6 +143,17 @@ def test_gated_layer_casts_another_down_projection():
     assert mlp.down.weight.dtype == mlp.down.bias.dtype == torch.bfloat16
 
 
+def test_norm_refuses_a_residual_of_another_shape():
+    """As many elements are not enough: rows of another order, or of another division into dimensions, are not x's."""
+    from quantization_amd import block_fp8 as F
+    x = torch.zeros(2, 3, 128)
+    for other in (x.view(3, 2, 128), x.view(6, 128), x[:, :1], x[0, 0]):
+        with pytest.raises(RuntimeError, match="residual must be"):
+            F.rms_norm_fp8(x, x[0, 0], 1e-6, residual=other)
+    with pytest.raises(RuntimeError, match="residual must be"):
+        F.rms_norm_fp8(x.view(6, 128), x[0, 0], 1e-6, residual=x)
+
+
 @pytest.mark.gpu
 def test_wrappers_refuse_wrong_tensors():
     from quantization_amd import block_fp8 as F
