@@ -39,7 +39,7 @@ struct Fp8Args {
     int N, K, kblocks;     // K: bytes between two rows of x and w, a multiple of 16
     int tiles_m, tiles_n;
     int kt_per_split;      // K-tiles each blockIdx.y slice sums; 0 = all, straight to `out`
-    int pitch;             // floats between two rows of a slab: N rounded up to 8 (columns past N hold zeros)
+    int pitch;             // floats between two rows of a slab: N rounded up to 8 (columns past N hold 0, or NaN in a row with a NaN code)
 };
 
 // A fragment of 16 rows and one K-tile: the lane's 16-byte chunks (lane >> 4) and 4 + (lane >> 4) of row lane & 15.
@@ -530,7 +530,7 @@ __global__ __launch_bounds__(64 * kWaves) void gemm_fp8_rows16_kernel(Fp8Args g)
         if (m >= g.M || n >= cols) continue;
         float v;
         if constexpr (GATED) v = gate_value<ACT>(sum_of(ch >> 4, m, ch & 15)) * sum_of(kEach + (ch >> 4), m, ch & 15);
-        else v = sum_of(ch >> 4, m, ch & 15) + (g.bias && !g.kt_per_split ? g.bias[n] : 0.f);
+        else v = n < g.N ? sum_of(ch >> 4, m, ch & 15) + (g.bias && !g.kt_per_split ? g.bias[n] : 0.f) : 0.f;   // (0 behind a slab's row)
         store_value<OUT>(out, static_cast<int64_t>(m) * cols + n, v);
     }
 }

@@ -673,6 +673,25 @@ def test_few_rows_of_any_length(m, n, k):
     check_gated(m, n, k, "silu")
 
 
+@pytest.mark.parametrize("m,n,k", [(2, 33, 16385), (16, 515, 16399), (1, 13, 28671), (2, 33, 16384), (40, 75, 3344)])
+def test_slab_columns_past_the_last_are_zero(m, n, k):
+    """A sliced product's slabs have rows of whole vectors; what is behind their last column is 0, whichever kernel wrote them."""
+    from quantization_amd import _native, block_fp8 as F
+    L = _native.lib()
+    q, s = F.quantize_blocks_fp8(rand(m, k, torch.float32, 1).cuda())
+    w, ws = F.quantize_weight_fp8(rand(n, k, torch.float32, 2).cuda())
+    need = L.miq_gemm_fp8_workspace(m, n, k, _native.MIQ_F32)
+    pitch = (n + 7) // 8 * 8
+    padded = 0 if k % 16 == 0 or m <= 16 else (m + n) * ((k + 15) // 16 * 16)
+    assert need > padded, "not sliced"
+    assert padded == 0 and need % (4 * m * pitch) == 0
+    work, out = torch.full((need,), 0xFF, dtype=torch.uint8, device="cuda"), torch.empty(m, n, device="cuda")
+    assert L.miq_gemm_fp8(q.data_ptr(), s.data_ptr(), w.data_ptr(), ws.data_ptr(), m, n, k, None, out.data_ptr(), _native.MIQ_F32,
+                          work.data_ptr(), need, torch.cuda.current_stream().cuda_stream) == 0
+    slabs = work.view(torch.float32).view(-1, m, pitch)
+    assert slabs.shape[0] > 1 and not bool(slabs[:, :, n:].any()) and bool(torch.isfinite(slabs).all())
+
+
 @pytest.mark.parametrize("m,k", [(1, 77), (5, 1001), (40, 300), (16, 136), (33, 5001), (3, 20001)])
 def test_nothing_behind_the_last_row(m, k):
     """Outputs through the C ABI, inside buffers of a known pattern: what lies behind them stays."""
