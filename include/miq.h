@@ -422,8 +422,10 @@ int miq_rms_norm_fp8(const void* x, const void* residual, const void* weight, in
  * MIQ_F32 | MIQ_F16 | MIQ_BF16.  x, w and out are 16-byte aligned.  K may be any; where it is no multiple of 16, operands of more
  * than 16 rows are copied to padded rows in the workspace first.
  * Sums are fp32, rounded once to out_dtype.  16-bit outputs of more than 16 rows are summed by the matrix cores' 8-bit
- * instruction, which drops of each product what lies below 2^-13 of the largest among eight neighbouring ones (3e-5 of a
- * result on layers' operands, a hundredth of the output's own rounding); every other product keeps 24 bits throughout.
+ * instruction, which drops of each product what lies below 2^-13 of the largest among eight neighbouring ones: 3e-5 of the
+ * outputs' root mean square on layers' operands, beside 1.7e-3 of a bf16 output's own rounding and 2.1e-4 of an fp16 one's.  fp32
+ * outputs, and products of at most 16 rows, keep 24 bits throughout (so a row's result may differ in this way between a call of 16
+ * rows and one of 17); a caller who wants them behind a 16-bit result takes an fp32 output and rounds that.
  * The product of two scales has to be a finite fp32 number.
  * M, N below 2^31, K below 2^22, at most 2^22 tiles of 64 x 64 outputs, N up to 2^26 where M is at most 16 (MIQ_ERANGE
  * otherwise).

@@ -56,7 +56,9 @@ def rms_norm_fp8(x, weight, eps=1e-6, residual=None):
 
 
 def linear_fp8(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16):
-    """x [..., K] codes with their scales, times w [N, K] codes with theirs, plus bias [N] -> [..., N] of out_dtype."""
+    """x [..., K] codes with their scales, times w [N, K] codes with theirs, plus bias [N] -> [..., N] of out_dtype.  Sums of more
+    than 16 rows for a 16-bit out_dtype are off by some 3e-5 of the outputs' root mean square beside the output's own rounding
+    (bfloat16 1.7e-3, float16 2.1e-4); float32 keeps 24 bits throughout, at half the matrix rate."""
     y = _native.gemm_fp8(_rows(x), x_scale, w, w_scale, bias, out_dtype)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[-1])
 

@@ -9,12 +9,12 @@
 //
 // Which instruction.  v_mfma_f32_16x16x128_f8f6f4 takes the codes as they are, a block in one instruction; but it (and the
 // 16x16x32 fp8 form) aligns the products of eight neighbouring k to the largest of the eight and drops what lies below 2^-13
-// of it (measured: 2^16 + 2^2 gives 2^16 where 2^16 + 2^3 is right; across groups of eight it keeps 24 bits).  On layers'
-// operands that is 3e-5 of the result, a hundred times an fp32 sum's error.  v_mfma_f32_16x16x32_bf16 keeps 24 bits
-// throughout (1e-8 on the same operands), and e4m3 widens to bf16 exactly (v_cvt_scalef32_pk_bf16_fp8, two codes an
-// instruction), at half the rate.  So 16-bit outputs, whose own rounding is 60 to 100 times coarser, take the 8-bit
-// instruction; fp32 outputs, the gated product (its scales are fp32) and products of at most 16 rows (which the weight's
-// stream bounds in either form) widen.
+// of it (measured: 2^16 + 2^3 comes out right, 2^16 + 2^2 as 2^16; across groups of eight it keeps 24 bits).  On layers'
+// operands that is 3e-5 of the outputs' root mean square, a hundred times an fp32 sum's error.  v_mfma_f32_16x16x32_bf16 keeps 24
+// bits throughout (1e-8 on the same operands), and e4m3 widens to bf16 exactly (v_cvt_scalef32_pk_bf16_fp8, two codes an
+// instruction), at half the rate.  So 16-bit outputs, whose own rounding is coarser (bf16 1.7e-3, 57 times as coarse; fp16 2.1e-4,
+// seven times), take the 8-bit instruction; fp32 outputs, the gated product (its scales are fp32) and products of at most 16 rows
+// (which the weight's stream bounds in either form) widen.
 //
 // What a block's scale costs: an accumulator is written by the vector unit once a K-tile, one fused multiply-add an output,
 // beside the matrix instructions; a product with one scale for a whole tensor has none of that.  The 16 x 16 instructions
@@ -187,8 +187,8 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs a) {
 }
 
 // The gate's activation.  The logistic function is the hardware's power of two and reciprocal (one unit each): the rounded
-// argument of a large exponent costs its result some units, where the result is far below 1 and is multiplied by the gate,
-// so that the activation is within a few units of the gate's own size.  (With the library's exponential and an IEEE
+// argument costs an exponential of a large gate |g| / 2 units, so that the activation is within |g| / 2 + 5 units of its own size
+// (40 at g = -70, under 1e-5 of it, beside an e4m3 code's half step of 6e-2).  (With the library's exponential and an IEEE
 // division the epilogue of a 256 x 128 tile took 11 us of vector instructions, a tenth of a K of 4096.)
 // GELU's 1 + erf(g / sqrt 2) is erfc(-g / sqrt 2): of a negative gate the sum would leave what rounding leaves of 1 - 1 (4% off at
 // g = -5, nothing at -5.5), and a block of negative gates takes its scale and every code from it.  (4096x14336x4096 861 us, with the
