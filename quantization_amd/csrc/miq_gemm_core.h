@@ -156,7 +156,7 @@ __device__ __forceinline__ uint32_t requant4_i8(float a, float b, float c, float
 #pragma clang fp contract(off)
     auto clamp = [](float y) { return __builtin_amdgcn_fmed3f(y, -128.0f, 127.0f); };
     const v2f magic{12582912.0f, 12582912.0f};
-    const v2f lo2 = v2f{clamp(a), clamp(b)} + magic, hi2 = v2f{clamp(c), clamp(d)} + magic;   // two packed additions
+    const v2f lo2 = v2f{clamp(a), clamp(b)} + magic, hi2 = v2f{clamp(c), clamp(d)} + magic;
     const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(lo2[1]), __float_as_uint(lo2[0]), 0x0c0c0400u);   // a.b0, b.b0, 0, 0
     const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(hi2[1]), __float_as_uint(hi2[0]), 0x04000c0cu);   // 0, 0, c.b0, d.b0
     return lo | hi;
@@ -173,7 +173,7 @@ __device__ __forceinline__ int8_t requant1_i8(float y) {
 // reference's tensor / tensor division; a scale of exactly 1 leaves y as it is.
 __device__ __forceinline__ float requant_div(float y, float scale) { return scale == 1.0f ? y : __fdiv_rn(y, scale); }
 
-// dequant1 on two values at once, as packed fp32 instructions (one rounding per step, no contraction).
+// dequant1 on two values at once (one rounding per step, no contraction; scalar instructions: the build turns packed fp32 off).
 __device__ __forceinline__ v2f dequant2(int a, int b, v2f bias, v2f alpha, v2f beta) {
 #pragma clang fp contract(off)
     v2f t{static_cast<float>(a), static_cast<float>(b)};
