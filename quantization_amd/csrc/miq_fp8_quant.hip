@@ -11,7 +11,7 @@ using namespace miq;
 
 // ---- activations: 1 x 128 ------------------------------------------------------------------------------------------
 // A workgroup of 16 sixteen-lane groups takes ROWS rows x (16 / ROWS) * kQuantPasses blocks.  Bound by HBM: 2048x14336 bf16
-// 16.0-16.5 us (5.4 TB/s read and written; a copy 4.9), fp32 28.0 (5.2); few rows by the launch, 2.5 us up to 64x14336.
+// 16.0-16.5 us (5.4 TB/s read and written; a copy 4.9), fp32 28.0-28.7 (5.2); few rows by the launch, 2.5 us up to 64x14336.
 template <int DT, bool VEC, int ROWS, int kQuantPasses>
 __global__ __launch_bounds__(256) void quantize_blocks_kernel(const void* __restrict__ x, int64_t M, int64_t K, int64_t kblocks,
                                                               int64_t col_groups, uint8_t* __restrict__ q,
@@ -40,7 +40,9 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(const void* __rest
 
 // ---- weights: 128 x 128 --------------------------------------------------------------------------------------------
 // One workgroup a block: a thread holds eight columns of eight rows (64 values) in registers, so that the weight is read once.
-// Bound by HBM: 14336x4096 fp32 50 us (5.9 TB/s), bf16 32.8 (5.4); rows that start anywhere (14336x4095 fp32) 86.
+// Bound by HBM: 14336x4096 fp32 50 us (5.9 TB/s), bf16 31.3 (5.6).  Rows that start anywhere (14336x4095 fp32) take 86: a block's rows
+// begin and end inside cache lines, which the neighbouring block's workgroup, as a rule on another XCD, fetches and writes, too:
+// 292 MB read for 235, 73 written for 59, a third of the writes partial lines; 365 MB at 4.2 TB/s.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void quantize_weight_kernel(const void* __restrict__ w, int64_t N, int64_t K, int64_t kblocks,
                                                               uint8_t* __restrict__ q, float* __restrict__ scale) {
@@ -103,8 +105,9 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const void* __rest
 // ---- root-mean-square norm -----------------------------------------------------------------------------------------
 // h = x + residual (rounded to the type it is stored in, so that the norm is the norm of the stored row), y = (h / rms) * g,
 // then y in blocks as above.  TPR threads a row; a row of at most TPR * 8 * VPT columns stays in registers between the sum
-// of squares and the codes (VPT > 0); a longer one is read twice (VPT = 0).  Bound by HBM: 8192x8192 bf16 with a residual 82.5 us
-// (5.7 TB/s), 8192x4096 44.3 (5.3), 1024x40000, read twice, 81.6 (3.5 TB/s of 7 bytes an element); one row 3.2 us, a launch.
+// of squares and the codes (VPT > 0); a longer one is read twice (VPT = 0).  Bound by HBM: 8192x8192 bf16 with a residual 83.1 us
+// (5.7 TB/s), 8192x4096 44.7 (5.3), 1024x40000, read twice, 82.4 (3.5 TB/s of 7 bytes an element); one row 3.7 us, a launch.  Some
+// hundred rows are all resident at once: beside the launch their bytes, 777x5000 fp16 6.9 us, 3.6 TB/s of the 3.2 us past one row's.
 template <int DT>
 __device__ __forceinline__ float round_to(float v) {
     if constexpr (DT == MIQ_BF16) return static_cast<float>(static_cast<__bf16>(v));
@@ -137,7 +140,9 @@ __device__ __forceinline__ void store8(void* base, int64_t index, int n, const f
             u32x4 v;
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = h[2 * i] | (static_cast<uint32_t>(h[2 * i + 1]) << 16);
-            __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(p));   // (8192 x 8192 with a residual: 95 us, 101 cached)
+            // (with a residual 8192x8192 83.1 us, cached 88.4; 2048x28672 89.6 and 92.3, 8192x2048 23.3 and 24.6; but 8192x4096 44.7 and
+            // 42.9, 1024x40000 82.4 and 79.4)
+            __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(p));
         } else if (!VEC) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -371,7 +376,7 @@ extern "C" int miq_rms_norm_fp8(const void* x, const void* residual, const void*
             const unsigned grid = static_cast<unsigned>(M);
             // Two vectors a thread where a row has as many threads (8192 x 8192 bf16 with a residual: 83 us as 512 threads of
             // two, 90 as 256 of four, 109 as 1024 of one; 8192x4096 44 as 256 of two, 49 as 512; 8192x2048 23.6 as 256 of one,
-            // 36 as 512); four keep rows of up to 32768 columns in registers (2048x28672 88 us, read twice 116).
+            // 36 as 512); four keep rows of up to 32768 columns in registers (2048x28672 90 us, read twice 116).
             if (cols <= 256 * 8) rms_norm_kernel<DT, V, 256, 1><<<grid, 256, 0, as_stream(stream)>>>(a);
             else if (cols <= 256 * 16) rms_norm_kernel<DT, V, 256, 2><<<grid, 256, 0, as_stream(stream)>>>(a);
             else if (cols <= 512 * 16) rms_norm_kernel<DT, V, 512, 2><<<grid, 512, 0, as_stream(stream)>>>(a);

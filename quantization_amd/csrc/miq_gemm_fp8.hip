@@ -1064,7 +1064,10 @@ Fp8Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated, bool native) {
     if (M <= 16) {
         // K in slices of at least eight K-tiles where the columns give few workgroups and K is long enough to pay for the second
         // launch: 1x512x28672 18.3 us whole, 8.0 in eight slices, 1x512x14336 11.2 and 6.6 (and 4 us more of the host), 1x2048x8192
-        // 7.4 and 8.3.  A gated product has its second launch anyway and would have a third (8x2048x4096 10.7 us, sliced 12.9).
+        // 7.4 and 8.3.  (In a captured graph, where a launch is no time of the host, 14336 columns of K would be worth slicing, too.)
+        // A gated product is never sliced, whatever K is: tried was a launch for each weight's slabs and one that joins them, three
+        // in all (8x2048x4096 12.9 us for 10.7).  Both weights' slabs from one launch, joined by the second, has not been built: the
+        // narrow and long products run on N / 16 workgroups (1x512x14336 19.3 us, 4x1024x8192 14.4; the bytes of either are 3).
         const int64_t groups = ceil_div(N, 16);
         if (!gated && groups < 192 && nt >= 128) {
             int64_t splits = kCus / groups;
